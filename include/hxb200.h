@@ -48,8 +48,11 @@ typedef enum hxb_dtype_e {
   HXB_DTYPE_I8 = 2,
 } hxb_dtype_t;
 
-/* Device status bits (hxb_device_status). */
+/* Device status bits (hxb_device_status): a bounded wait of a kernel gave up;
+ * an index that a kernel read from device memory (a block id, a slot, a
+ * length) was outside its range and was not followed. */
 #define HXB_DEVICE_STATUS_TIMEOUT 1
+#define HXB_DEVICE_STATUS_BAD_INDEX 2
 
 /* ABI version compiled into the library (HXB_ABI_VERSION). */
 int hxb_abi_version(void);
@@ -458,6 +461,95 @@ hxb_status_t hxb_decoder_block_w8a16_cached(const hxb_decoder_w8_t* w,
                                             void* v_cache, int64_t cache_rows,
                                             void* workspace,
                                             size_t workspace_bytes, void* stream);
+
+/* ---- Paged KV cache: batches of requests with different lengths ----------
+ * The reference's KV-cache models keep one length and one contiguous cache
+ * per batch (integration_tests/models/kv_cache.py:91-112). The entries below
+ * serve requests of different lengths from one pool of blocks:
+ *   k_cache, v_cache  [num_blocks, kv_heads, block_rows, head_dim] f16; the
+ *                     blocks of both are block_stride elements apart (a
+ *                     multiple of 8, at least kv_heads * block_rows *
+ *                     head_dim), so both may be views of one array.
+ *                     block_rows is a power of two from 16 to 1024.
+ *   block_table       [batch, table_ld] int32, table_cols of them used: cache
+ *                     row r of request b is row r % block_rows of block
+ *                     block_table[b][r / block_rows].
+ * Lengths and tables are read on the GPU, so a captured graph follows them. A
+ * value outside its range (a block id, a slot, a length, a row start) is not
+ * followed: it sets HXB_DEVICE_STATUS_BAD_INDEX and the results it would have
+ * reached are unspecified. */
+
+/* The tables of one step, for requests with cached_lens[b] rows in the cache
+ * and new_lens[b] tokens to add (batch <= 16384, block_rows >= 1):
+ *   q_start  [batch + 1]   first row of each request among the step's tokens
+ *   kv_lens  [batch]       cached_lens + new_lens; may be cached_lens itself
+ *   block_table            entries of the blocks a request begins in this step
+ *                          are taken from free_blocks[*cursor ..] in request
+ *                          order; the other entries are left as they are
+ *   slots    [max_tokens]  block * block_rows + row of each new token, -1
+ *                          behind the last one
+ *   cursor_out [2]         the cursor behind the blocks taken (may be cursor),
+ *                          then how many blocks the free list was short of:
+ *                          tokens without a block get slot -1 and table entry
+ *                          -1
+ * A request is cut at table_cols * block_rows rows, the batch at max_tokens
+ * tokens (both set HXB_DEVICE_STATUS_BAD_INDEX). No other output may overlap
+ * an input. */
+hxb_status_t hxb_paged_tables(const int32_t* cached_lens, const int32_t* new_lens,
+                              int64_t batch, int64_t block_rows,
+                              const int32_t* free_blocks, int64_t num_free,
+                              const int32_t* cursor, int32_t* block_table,
+                              int64_t table_ld, int64_t table_cols,
+                              int32_t* q_start, int32_t* kv_lens, int64_t* slots,
+                              int64_t max_tokens, int32_t* cursor_out, void* stream);
+
+/* hxb_kv_cache_write_f16 through a slot map:
+ *   k_cache[slots[t] / block_rows, h, slots[t] % block_rows, :] =
+ *       k_src[t, h*D : (h+1)*D]
+ * and V alike, for t < tokens. Sources are row-major [tokens, ld_src] f16 with
+ * 16-byte aligned rows. A negative slot writes nothing (padded rows); equal
+ * slots leave either row. head_dim is a multiple of 8. */
+hxb_status_t hxb_kv_cache_write_paged_f16(const void* k_src, const void* v_src,
+                                          int64_t ld_src, const int64_t* slots,
+                                          int64_t tokens, void* k_cache, void* v_cache,
+                                          int64_t block_stride, int64_t num_blocks,
+                                          int64_t kv_heads, int64_t block_rows,
+                                          int64_t head_dim, void* stream);
+
+/* Grouped-query attention of a batch over a paged cache, behind a prefix that
+ * all its requests share and that is read once for all of them. Rows
+ * [q_start[b], q_start[b + 1]) of Q and O are the tokens of request b; they
+ * attend to
+ *   - the prefix_len rows of the prefix's blocks (prefix_table, all visible),
+ *   - the first kv_lens[b] rows of the request's own blocks (block_table);
+ *     causal != 0 hides own row j > kv_lens[b] - n + i from token i of n (the
+ *     tokens are the last cached rows).
+ *   Q, O  [total_q, q_heads, head_dim] f16, rows ldq / ldo elements apart
+ *         (multiples of 8; Q may be columns of a fused QKV projection)
+ * Query head h reads KV head h / (q_heads / kv_heads), at most 128 query heads
+ * per KV head; head_dim 64 or 128. prefix_len 0 runs without a prefix. Tokens
+ * that see no key are 0; rows of O before q_start[0] and from
+ * q_start[batch] on are left as they are. Cache rows behind a length are not
+ * used, whatever they hold; rows within it must be finite where a token of
+ * the request may not see them. f32 scores, statistics and sums; P is rounded
+ * to f16 for the second product.
+ * max_q_len: the most tokens a request is expected to have (1 for decode).
+ * Requests may have more; it chooses kernels, not results. workspace:
+ * hxb_attention_paged_workspace_bytes(...) bytes, 16-byte aligned, no initial
+ * contents; calls that share one must be ordered (one stream). */
+hxb_status_t hxb_attention_paged_f16(
+    const void* Q, int64_t ldq, void* O, int64_t ldo, const int32_t* q_start,
+    const int32_t* kv_lens, int64_t batch, int64_t total_q, int64_t max_q_len,
+    const void* k_cache, const void* v_cache, int64_t block_stride, int64_t num_blocks,
+    int64_t block_rows, const int32_t* block_table, int64_t table_ld, int64_t table_cols,
+    const int32_t* prefix_table, int64_t prefix_len, int64_t q_heads, int64_t kv_heads,
+    int64_t head_dim, float scale, int causal, void* workspace, size_t workspace_bytes,
+    void* stream);
+
+/* Workspace of hxb_attention_paged_f16 on the current device (0 if the extents
+ * are invalid or total_q is 0). */
+size_t hxb_attention_paged_workspace_bytes(int64_t total_q, int64_t q_heads,
+                                           int64_t head_dim, int64_t prefix_len);
 
 #ifdef __cplusplus
 }

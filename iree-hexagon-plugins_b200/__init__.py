@@ -12,8 +12,12 @@ from . import compiler, hal, sharded
 from .dispatch import (DecoderBlockW8, attention, attention_bshd, attention_gqa,
                        attention_gqa_workspace_bytes, device_status, kv_cache_write, matmul,
                        matmul_w8a16, rmsnorm, rope_, swiglu, w8a16_workspace)
+from .paged import (attention_paged, attention_paged_workspace_bytes, kv_cache_write_paged,
+                    paged_tables)
 
 __all__ = ["compiler", "hal", "sharded", "HxbError", "DecoderBlockW8", "attention", "attention_bshd",
-           "attention_gqa", "attention_gqa_workspace_bytes", "device_status",
-           "kv_cache_write", "matmul", "matmul_w8a16", "rmsnorm", "rope_", "swiglu",
+           "attention_gqa", "attention_gqa_workspace_bytes", "attention_paged",
+           "attention_paged_workspace_bytes", "device_status", "kv_cache_write",
+           "kv_cache_write_paged", "paged_tables",
+           "matmul", "matmul_w8a16", "rmsnorm", "rope_", "swiglu",
            "w8a16_workspace", "_native"]

@@ -75,6 +75,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                        c_i64, c_i64, c_vp]),
     "hxb_decoder_block_w8a16": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
                                         c_size, c_vp]),
+    "hxb_paged_tables": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,
+                                 c_vp, c_vp, c_vp, c_i64, c_vp, c_vp]),
+    "hxb_kv_cache_write_paged_f16": (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
+                                             c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "hxb_attention_paged_f16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
+                                        c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp,
+                                        c_i64, c_i64, c_i64, c_i64, c_float, c_int, c_vp, c_size,
+                                        c_vp]),
+    "hxb_attention_paged_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
     # include/hxb200_hal.h: executable library
     "hxb_executable_library_query": (c_vp, [ctypes.c_uint32, c_vp]),
     # include/hxb200_hal.h: HAL runtime

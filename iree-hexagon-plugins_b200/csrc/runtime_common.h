@@ -55,6 +55,12 @@ hxb_status_t encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype,
                                const uint32_t* box,
                                CUtensorMapSwizzle swizzle);
 
+// Checks the description of a paged KV cache (paged_cache.cu); `what` names
+// the entry in the message.
+hxb_status_t check_paged_cache(const char* what, const void* k_cache, const void* v_cache,
+                               int64_t block_stride, int64_t num_blocks, int64_t kv_heads,
+                               int64_t block_rows, int64_t head_dim);
+
 inline bool aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }

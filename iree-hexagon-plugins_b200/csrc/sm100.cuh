@@ -20,8 +20,11 @@ namespace hxb {
 // hanging the GPU. Legitimate waits inside one launch are microseconds.
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s
 
-// Status bits written into the device status word on a failed wait.
+// Status bits written into the device status word: a failed wait, and an
+// index in device memory (a block id, a slot, a length) outside its range,
+// which the kernel did not follow.
 constexpr int kStatusTimeout = 1;
+constexpr int kStatusBadIndex = 2;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
@@ -200,6 +203,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map,
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_"
       "tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
+// 3-D form of tma_load_2d; x is the innermost coordinate.
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map,
+                                            uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_"
+      "tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
 

@@ -1,0 +1,124 @@
+"""Refusals of the paged-cache entries: bad arguments are answered on the host,
+before any device access (no GPU needed; the pointers are never followed)."""
+from __future__ import annotations
+
+import pytest
+
+A = 0x100000  # an aligned address
+
+
+def attention(lib, **kw):
+    a = dict(Q=A, ldq=1024, O=A, ldo=1024, q_start=A, kv_lens=A, batch=2, total_q=2, max_q=1, k=A, v=A,
+             stride=2 * 16 * 128, blocks=8, rows=16, table=A, table_ld=4, cols=4, ptable=A, prefix=20,
+             q_heads=8, kv_heads=2, D=128, scale=0.1, causal=1, ws=A, ws_bytes=1 << 40, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.hxb_attention_paged_f16(*a.values())
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(D=96), 2, b"head dim 96"),
+    (dict(rows=48), 2, b"power of two"),
+    (dict(rows=8), 2, b"power of two"),
+    (dict(rows=2048, stride=2 * 2048 * 128), 2, b"power of two"),
+    (dict(q_heads=9), 1, b"multiple of kv_heads"),
+    (dict(q_heads=0), 1, b"multiple of kv_heads"),
+    (dict(kv_heads=0), 1, b"cache extents"),
+    (dict(q_heads=258), 2, b"query heads per KV head"),
+    (dict(batch=0), 1, b"batch"),
+    (dict(total_q=-1), 1, b"batch"),
+    (dict(prefix=-1), 1, b"extents"),
+    (dict(cols=5), 1, b"extents"),
+    (dict(cols=0), 1, b"extents"),
+    (dict(scale=0.0), 1, b"scale"),
+    (dict(scale=float("inf")), 1, b"scale"),
+    (dict(scale=float("nan")), 1, b"scale"),
+    (dict(stride=2 * 16 * 128 - 8), 1, b"block_stride"),
+    (dict(stride=2 * 16 * 128 + 4), 1, b"block_stride"),
+    (dict(k=A + 8), 1, b"16-byte"),
+    (dict(v=None), 1, b"null cache"),
+    (dict(Q=None), 1, b"null"),
+    (dict(ptable=None), 1, b"null"),
+    (dict(Q=A + 2), 1, b"16-byte"),
+    (dict(ldq=1028), 1, b"16-byte"),
+    (dict(ldo=512), 1, b"16-byte"),
+    (dict(total_q=1 << 29), 1, b"extents"),
+    (dict(blocks=0), 1, b"cache extents"),
+])
+def test_attention_paged_refuses(pkg, kw, status, text):
+    lib = pkg._native.load()
+    assert attention(lib, **kw) == status
+    assert text in lib.hxb_last_error_message()
+
+
+def test_attention_paged_without_tokens_is_nothing(pkg):
+    assert attention(pkg._native.load(), total_q=0, Q=None, O=None, ws=None, ws_bytes=0) == 0
+
+
+def tables(lib, **kw):
+    a = dict(cached=A, new=A, batch=2, rows=16, free=A, num_free=4, cursor=A, table=A, table_ld=4,
+             cols=4, q_start=A, kv_lens=A, slots=A, max_tokens=8, cursor_out=A, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.hxb_paged_tables(*a.values())
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(batch=0), b"requests"), (dict(batch=16385), b"requests"), (dict(rows=0), b"extents"),
+    (dict(cols=0), b"extents"), (dict(cols=5), b"extents"), (dict(max_tokens=-1), b"extents"),
+    (dict(num_free=-1), b"extents"), (dict(rows=1 << 20, cols=1 << 12, table_ld=1 << 12), b"extents"),
+    (dict(cached=None), b"null"), (dict(free=None), b"null"), (dict(slots=None), b"null"),
+    (dict(cursor_out=None), b"null"),
+])
+def test_paged_tables_refuses(pkg, kw, text):
+    lib = pkg._native.load()
+    assert tables(lib, **kw) == 1
+    assert text in lib.hxb_last_error_message()
+
+
+def write(lib, **kw):
+    a = dict(k=A, v=A, ld=256, slots=A, tokens=3, kc=A, vc=A, stride=2 * 16 * 128, blocks=8, heads=2,
+             rows=16, D=128, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.hxb_kv_cache_write_paged_f16(*a.values())
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(rows=24), 2, b"power of two"), (dict(D=12), 2, b"head_dim"), (dict(D=2048), 2, b"head_dim"),
+    (dict(tokens=-1), 1, b"token count"), (dict(k=None), 1, b"null"), (dict(slots=None), 1, b"null"),
+    (dict(ld=255), 1, b"16-byte"), (dict(ld=248), 1, b"16-byte"), (dict(v=A + 8), 1, b"16-byte"),
+    (dict(kc=A + 8), 1, b"16-byte"), (dict(stride=128), 1, b"block_stride"),
+    (dict(heads=0), 1, b"cache extents"),
+])
+def test_kv_cache_write_paged_refuses(pkg, kw, status, text):
+    lib = pkg._native.load()
+    assert write(lib, **kw) == status
+    assert text in lib.hxb_last_error_message()
+
+
+def test_workspace_query_of_invalid_extents_is_zero(pkg):
+    lib = pkg._native.load()
+    assert lib.hxb_attention_paged_workspace_bytes(0, 8, 128, 0) == 0
+    assert lib.hxb_attention_paged_workspace_bytes(4, 8, 96, 0) == 0
+    assert lib.hxb_attention_paged_workspace_bytes(4, 0, 128, 0) == 0
+    assert lib.hxb_attention_paged_workspace_bytes(4, 8, 128, -1) == 0
+
+
+def test_python_entries_refuse_before_the_library(pkg):
+    import torch
+    f16 = dict(dtype=torch.float16)
+    cache = torch.zeros(2, 1, 16, 64, **f16)
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.kv_cache_write_paged(torch.zeros(1, 64, **f16), torch.zeros(1, 64, **f16), cache, cache,
+                                 torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(ValueError, match="contiguous"):
+        pkg.kv_cache_write_paged(torch.zeros(1, 64, **f16), torch.zeros(1, 64, **f16),
+                                 cache.transpose(2, 3), cache.transpose(2, 3),
+                                 torch.zeros(1, dtype=torch.int64))
+    with pytest.raises(ValueError, match="f16"):
+        pkg.kv_cache_write_paged(torch.zeros(1, 64), torch.zeros(1, 64), cache.float(), cache.float(),
+                                 torch.zeros(1, dtype=torch.int64))
+    ints = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.paged_tables(ints, ints, ints, ints, ints[None], block_rows=16, max_tokens=1)
