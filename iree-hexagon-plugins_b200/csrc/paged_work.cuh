@@ -1,0 +1,393 @@
+// What the paged attention kernels (attention_paged.cu) share: the arguments of
+// a call, how its work is laid end to end and shared out, and where partial
+// results go.
+//
+// Work: a "segment" is one key set (the shared prefix, or the own keys of one
+// request), its tokens cut into row units of unit_tok tokens. For every KV head
+// and row unit it visits key blocks of 128. All of that is laid end to end in
+// units of one block -- prefix, request 0, request 1 ...; inside a segment KV
+// head by KV head, row unit by row unit -- and CTA i takes units [i S, (i + 1) S),
+// S = ceil(T / CTAs): equal shares whatever the lengths, which are read on the
+// GPU. The part of a row unit's blocks that falls to one CTA is an item;
+// a row unit cut between CTAs leaves one partial result per CTA.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "sm100.cuh"
+
+namespace hxb {
+
+constexpr int kBM = 128;  // rows per tile of the wide kernel
+constexpr int kBN = 128;  // keys per block
+constexpr int kBoxBytes = 128 * 64 * 2;  // 128 rows x 64 f16
+constexpr int kNarrowRows = 16;          // rows per unit of the narrow kernel
+constexpr float kMoveLog2 = 8.0f;        // the running maximum moves by more than 2^8
+constexpr int kEnd = -2;
+
+// One piece of work: `blocks` key blocks from block j0 of a row unit.
+struct Item {
+  int request;  // -1: the shared prefix; kEnd: no more work
+  int head;     // KV head
+  int tok0;     // first token of the row unit
+  int ntok;     // its tokens
+  int j0, blocks;
+  int keys;     // keys of the segment's key set
+  int pos0;     // last key that token tok0 sees (causal), else INT_MAX / 2
+  int slot;     // partial slot of a cut row unit, -1: it is whole here
+  int first, pieces;  // a cut row unit: slot of its first piece, and how many
+};
+static_assert(sizeof(Item) <= 64, "item record");
+
+struct PagedArgs {
+  const int* q_start;
+  const int* kv_lens;
+  const int* block_table;
+  const int* prefix_table;
+  const __half* Q;  // the narrow kernel copies Q without TMA
+  __half* O;
+  long long ldq, ldo, table_ld;
+  int total_q, batch, q_heads, kv_heads, group;
+  int unit_tok;            // tokens per row unit
+  int min_tok, max_tok;    // this kernel takes the requests of that many tokens
+  int prefix_here;         // and the prefix
+  int tile_tok, box_tok;   // wide kernel: tokens per 128-row tile and per Q box
+  int table_cols, num_blocks, rows_log2;
+  int prefix_len;
+  int causal;
+  float c;  // scale * log2(e)
+  // Partial results, f32, normalised, with their log2-sum-exp2. Packed row
+  // pr = token * group + head-in-group of KV head h. Four columns of a row lie
+  // together and the rows of a tile side by side, so that threads that hold a
+  // row each write and read whole lines:
+  //   cut row units  cut_o[kernel][slot][D / 4][rows][4], slot = 2 CTA (the
+  //                  CTA's first item) or 2 CTA + 1 (its last); rows = 256
+  //                  (wide, kernel 0) or 16 (narrow, kernel 1)
+  //   whole ones     whole_o[set][h][D / 4][total_q * group][4], set = 0 own
+  //                  keys, 1 prefix
+  // info[set][h][pr]: {slot of the first piece (narrow: + kNarrowSlot),
+  // pieces | row in the slot << 16}
+  float* cut_o[2];
+  float* cut_lse[2];
+  float* whole_o[2];
+  float* whole_lse[2];
+  int2* info[2];
+  int ctas[2];
+  int* status;
+};
+constexpr int kNarrowSlot = 1 << 30;
+
+// Position in a ring of N slots, counted in uses.
+template <int N>
+struct Ring {
+  uint32_t n = 0;
+  __device__ __forceinline__ int slot() const { return n % N; }
+  __device__ __forceinline__ uint32_t parity() const { return (n / N) & 1; }
+};
+
+__device__ __forceinline__ uint64_t kmajor_desc(uint32_t base) {
+  return make_smem_desc(base, 16, 1024, kLayoutSwizzle128);
+}
+__device__ __forceinline__ uint64_t vmajor_desc(uint32_t base) {
+  return make_smem_desc(base, kBoxBytes, 1024, kLayoutSwizzle128);
+}
+// K-major 16-element K step kk of a tile of boxes of `box` bytes x 64 columns,
+// in descriptor address units.
+__device__ __forceinline__ constexpr uint64_t kstep(int kk, int box = kBoxBytes) {
+  return (uint64_t)(((kk >> 2) * box + (kk & 3) * 32) >> 4);
+}
+
+__device__ __forceinline__ int clamp_token(const PagedArgs& a, int b) {
+  return min(max(a.q_start[b], 0), a.total_q);
+}
+
+struct Segment {
+  int tok, n, keys;
+  int units;       // row units
+  int work;        // blocks of one KV head over all row units
+  bool causal;
+};
+
+// Keys that the last token of row unit u sees.
+__device__ __forceinline__ int unit_keys(const PagedArgs& a, const Segment& s, int u) {
+  if (!s.causal) return s.keys;
+  const int last = min((u + 1) * a.unit_tok, s.n);
+  return max(0, min(s.keys, s.keys - s.n + last));
+}
+
+__device__ __forceinline__ int unit_blocks(const PagedArgs& a, const Segment& s, int u) {
+  return max(1, (unit_keys(a, s, u) + kBN - 1) / kBN);  // an empty unit still writes its rows
+}
+
+// sum_{i < n} floor((a i + b) / m), by the Euclidean algorithm on (a, m): whole
+// multiples of m leave the sum in closed form, and what is left counts the
+// lattice points under a line, which swapping the axes turns into a shorter sum.
+__device__ __forceinline__ long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  long long sum = 0;
+  while (true) {
+    sum += (long long)n * (n - 1) / 2 * (a / m) + (long long)n * (b / m);
+    a %= m;
+    b %= m;
+    const unsigned top = a * n + b;  // (a, b < m <= 256: below 2^32)
+    if (top < m) return sum;
+    n = top / m;
+    b = top % m;
+    const unsigned t = m;
+    m = a;
+    a = t;
+  }
+}
+
+constexpr int kMostWork = 1 << 30;  // blocks of one call (saturated above)
+
+// Blocks of the first `units` row units of one KV head.
+__device__ __forceinline__ int blocks_before(const PagedArgs& a, const Segment& s, int units) {
+  if (units <= 1) return units == 0 ? 0 : unit_blocks(a, s, 0);
+  if (!s.causal) return (int)min((long long)units * unit_blocks(a, s, 0), (long long)kMostWork);
+  // unit u < units - 1 sees d + (u + 1) T keys: none up to u = dark (one block
+  // each), then one block per begun 128
+  const int T = a.unit_tok, d = s.keys - s.n, full = units - 1;
+  const int dark = d < 0 ? min(full, (-d) / T) : 0;
+  long long sum = dark;
+  if (full > dark) sum += floor_sum(full - dark, kBN, T, d + (dark + 1) * T + kBN - 1);
+  return (int)min(sum + unit_blocks(a, s, full), (long long)kMostWork);
+}
+
+__device__ __forceinline__ Segment own_segment(const PagedArgs& a, int b) {
+  Segment s;
+  s.tok = clamp_token(a, b);
+  s.n = max(clamp_token(a, b + 1) - s.tok, 0);
+  if (s.n < a.min_tok || s.n > a.max_tok) s.n = 0;  // the other kernel's
+  s.keys = (int)min((long long)max(a.kv_lens[b], 0), (long long)a.table_cols << a.rows_log2);
+  s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
+  s.causal = a.causal != 0;
+  s.work = s.units ? blocks_before(a, s, s.units) : 0;
+  return s;
+}
+
+__device__ __forceinline__ Segment prefix_segment(const PagedArgs& a) {
+  Segment s;
+  s.tok = clamp_token(a, 0);
+  s.n = a.prefix_here ? max(clamp_token(a, a.batch) - s.tok, 0) : 0;
+  s.keys = a.prefix_len;
+  s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
+  s.causal = false;
+  s.work = (int)min((long long)s.units * ((s.keys + kBN - 1) / kBN), (long long)kMostWork);
+  return s;
+}
+
+// A CTA's share of the work: units [lo, hi), `per` units per CTA.
+struct Share {
+  int lo, hi, per;
+};
+template <int THREADS>
+struct ShareSmem {
+  long long sum[THREADS / 32];
+  Segment seg;  // where the share begins: segment, request (-1: the prefix) and
+  int b, off;   // unit within the segment
+};
+
+// Every thread sums the work of a run of requests; a block scan gives the total,
+// and the thread that holds the CTA's first unit notes its segment. Called by
+// the whole block.
+template <int THREADS>
+__device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREADS>& sm) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Segment pre = prefix_segment(a);
+  const int each = a.min_tok <= a.max_tok ? (a.batch + THREADS - 1) / THREADS : 0;
+  const int b0 = min((int)threadIdx.x * each, a.batch), b1 = min(b0 + each, a.batch);
+  long long mine = 0;
+  Segment s;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    s = own_segment(a, b);
+    mine += (long long)s.work * a.kv_heads;
+  }
+  long long scan = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) sm.sum[warp] = scan;
+  __syncthreads();
+  const long long pre_work = (long long)pre.work * a.kv_heads;
+  long long total = pre_work, base = pre_work;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w == warp) base = total;
+    total += sm.sum[w];
+  }
+  base += scan - mine;
+  Share r{0, 0, 1};
+  if (total >= kMostWork) {  // (hours of work: not started)
+    if (threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
+    return r;
+  }
+  r.per = max(1, ((int)total + (int)gridDim.x - 1) / (int)gridDim.x);
+  r.lo = min((int)blockIdx.x * r.per, (int)total);
+  r.hi = min(r.lo + r.per, (int)total);
+  if (r.lo < r.hi) {
+    if (r.lo >= base && r.lo < base + mine) {
+      int at = (int)base;
+#pragma unroll 1
+      for (int b = b0; b < b1; ++b) {
+        if (each > 1) s = own_segment(a, b);
+        const int w = s.work * a.kv_heads;
+        if (r.lo < at + w) {
+          sm.b = b;
+          sm.off = r.lo - at;
+          sm.seg = s;
+          break;
+        }
+        at += w;
+      }
+    } else if (threadIdx.x == 0 && r.lo < pre_work) {
+      sm.b = -1;
+      sm.off = r.lo;
+      sm.seg = pre;
+    }
+  }
+  __syncthreads();
+  return r;
+}
+
+// mbar_wait with its loop out of line: the roles of these kernels wait in many
+// places, and what runs once per item should not be fetched anew for each.
+static __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                              int* status) {
+  return mbar_wait(bar, parity, FailState{abort, status});
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const FailState& fs) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return wait_slow(bar, parity, fs.abort, fs.status);
+}
+
+// Publishes the CTA's items, one after the other, into a ring of N records (one
+// thread). item_empty[] collects one arrival of every reader of a record.
+// OUT_OF_LINE: wait through wait_bar (not in a kernel that moves registers with
+// setmaxnreg, where the compiler cannot place a call).
+template <int N, bool OUT_OF_LINE, int THREADS>
+__device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
+                                         const ShareSmem<THREADS>& sm, Item* items,
+                                         uint64_t* item_full, uint64_t* item_empty,
+                                         const FailState& fs) {
+  Ring<N> out;
+  int b = -1, h = 0, u = 0, j = 0;
+  int pos = sh.lo;
+  Segment s;
+  s.work = 0;
+  s.units = 0;
+  // The lengths of the following segments are read again, one at a time. Lengths
+  // that another stream changes meanwhile (a caller's mistake) must not lead out
+  // of the tables: a position that is none ends the work.
+  if (sh.lo < sh.hi) {
+    s = sm.seg;
+    b = sm.b;
+    int off = max(sm.off, 0);
+    if (s.work > 0) {
+      h = min(off / s.work, a.kv_heads);
+      off = min(off - h * s.work, s.work - 1);
+      int above = s.units;  // blocks_before(u) <= off < blocks_before(above)
+      while (above - u > 1) {
+        const int mid = (u + above) >> 1;
+        if (blocks_before(a, s, mid) <= off) u = mid;
+        else above = mid;
+      }
+      if (u) off -= blocks_before(a, s, u);
+      j = off;
+    }
+  }
+#pragma unroll 1
+  while (true) {
+    Item item;
+    item.request = kEnd;
+    item.blocks = 0;
+    const int kb = unit_blocks(a, s, u);
+    if (pos < sh.hi && s.work > 0 && h < a.kv_heads && u < s.units && j < kb) {
+      const int take = min(kb - j, sh.hi - pos);
+      item.request = b;
+      item.head = h;
+      item.tok0 = s.tok + u * a.unit_tok;
+      item.ntok = min(s.n - u * a.unit_tok, a.unit_tok);
+      item.j0 = j;
+      item.keys = s.keys;
+      item.pos0 = s.causal ? s.keys - s.n + u * a.unit_tok : INT32_MAX / 2;
+      const bool empty = s.keys == 0 || item.pos0 + item.ntok <= 0;
+      item.blocks = empty ? 0 : take;
+      item.slot = -1;
+      item.pieces = 1;
+      item.first = 0;
+      if (j != 0 || take != kb) {
+        const int begin = pos - j, c0 = begin / sh.per;
+        item.first = 2 * c0 + (c0 * sh.per != begin);
+        item.pieces = (begin + kb - 1) / sh.per - c0 + 1;
+        item.slot = 2 * (int)blockIdx.x + (pos != sh.lo);
+      }
+      pos += take;
+      j = 0;
+      if (pos < sh.hi && ++u == s.units) {
+        u = 0;
+        if (++h == a.kv_heads) {
+          h = 0;
+          s.work = 0;
+          while (s.work == 0 && b + 1 < a.batch) s = own_segment(a, ++b);
+        }
+      }
+    }
+    uint64_t* free_slot = &item_empty[out.slot()];
+    const uint32_t parity = out.parity() ^ 1;
+    if (!(OUT_OF_LINE ? wait_bar(free_slot, parity, fs) : mbar_wait(free_slot, parity, fs))) return;
+    items[out.slot()] = item;
+    mbar_arrive(&item_full[out.slot()]);
+    ++out.n;
+    if (item.request == kEnd) return;
+  }
+}
+
+// Loads this lane's boxes of one 128-key K or V tile (a whole warp calls it): a
+// box is up to 128 rows of one cache block and 64 columns. Rows from item.keys
+// on are zeros where a whole box is (an out-of-range block fills with zeros).
+template <int D>
+struct TileLoader {
+  static constexpr int kBoxes = D / 64;
+  int lane, boxes, row, half;
+  __device__ __forceinline__ TileLoader(const PagedArgs& a, int lane_) : lane(lane_) {
+    const int page_rows = min(1 << a.rows_log2, kBN);
+    boxes = kBN / page_rows * kBoxes;  // at most 16
+    row = lane / kBoxes * page_rows;
+    half = lane % kBoxes;
+  }
+  // the cache block of this lane's box of key block j
+  __device__ __forceinline__ int block_of(const PagedArgs& a, int keys, const int* table,
+                                          int j) const {
+    const int key = j * kBN + row;
+    if (lane >= boxes || key >= keys) return a.num_blocks;
+    const int id = table[key >> a.rows_log2];
+    if (id >= 0 && id < a.num_blocks) return id;
+    atomicOr(a.status, kStatusBadIndex);
+    return a.num_blocks;
+  }
+  __device__ __forceinline__ void load(const PagedArgs& a, int head, const CUtensorMap* map,
+                                       void* tile, uint64_t* bar, int j, int block) const {
+    if (lane == 0) mbar_arrive_expect_tx(bar, kBN * D * 2);
+    __syncwarp();
+    const int in = (j * kBN + row) & ((1 << a.rows_log2) - 1);
+    if (lane < boxes)
+      tma_load_3d(static_cast<uint8_t*>(tile) + half * kBoxBytes + row * 128, map, bar, 64 * half,
+                  (head << a.rows_log2) + in, block);
+  }
+};
+
+// Block table of an item.
+__device__ __forceinline__ const int* item_table(const PagedArgs& a, const Item& item) {
+  return item.request < 0 ? a.prefix_table : a.block_table + (long long)item.request * a.table_ld;
+}
+// Rows of the item's last key block that exist; a block with fewer than 128 gets
+// the others of its V tile zeroed (their P is 0, but 0 * NaN is not).
+__device__ __forceinline__ int tail_rows(const Item& item) {
+  return item.keys - (item.j0 + item.blocks - 1) * kBN;
+}
+
+}  // namespace hxb
