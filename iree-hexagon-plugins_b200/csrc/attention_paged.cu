@@ -36,6 +36,11 @@ namespace {
 // kernel, which reads it once per 16 rows (from L2 after the first).
 constexpr int kNarrowPrefixRows = 64;
 
+// What a row unit of the wide kernel costs on top of its key blocks (Q, the first
+// softmax without an overlapping product, the epilogue), in blocks. The narrow
+// kernel hides it behind the loads of its other CTA.
+constexpr int kWideUnitCost = 2;
+
 // Merges the partials of every row: a block has 32 packed rows of one KV head
 // (lane = row) and 64 columns (warp = 8 of them), so that partials, which lie
 // row by row in groups of four columns, are read in whole lines. A row has one
@@ -68,7 +73,8 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
   const int tok = (int)(pr / a.group);
   if (tok < clamp_token(a, 0) || tok >= clamp_token(a, a.batch)) return;
   const int n_own = own.y & 0xffff, n_pre = pre.y & 0xffff;
-  if (a.prefix_len == 0 && n_own == 1) return;  // written by the attention kernel
+  const bool prefix = a.prefix_len > 0 && !(own.x & kWithPrefix);
+  if (!prefix && n_own == 1) return;  // written by the attention kernel
   float m = -INFINITY, sum = 0.0f;
   float acc[8];
 #pragma unroll
@@ -76,11 +82,10 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
   bool wrong = false;
   auto merge = [&](int set, int2 info, int n) {
     const bool narrow = (info.x & kNarrowSlot) != 0;
-    const int first = info.x & ~kNarrowSlot, prow = info.y >> 16;
+    const int first = info.x & (kWithPrefix - 1), prow = info.y >> 16;
     const int rows = narrow ? kNarrowRows : 256;
     // (records left unwritten by a launch that gave up on a wait)
-    if (n < 1 || info.x < 0 || (unsigned)prow >= (unsigned)rows ||
-        2 * ((first >> 1) + n) > 2 * a.ctas[narrow]) {
+    if (n < 1 || info.x < 0 || (unsigned)prow >= (unsigned)rows || first + n > a.ctas[narrow]) {
       wrong = true;
       return;
     }
@@ -103,7 +108,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
           pitch = R * 4;
           lse[i] = a.whole_lse[set][at];
         } else {
-          const long long slot = p == 0 ? first : 2 * ((first >> 1) + p);
+          const long long slot = p == 0 ? 2 * first + 1 : 2 * (first + p);
           src = cut_o + (slot * D + v0 * 4) * rows + prow * 4;
           pitch = rows * 4;
           lse[i] = cut_lse[slot * rows + prow];
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
     }
   };
   merge(0, own, n_own);
-  if (a.prefix_len > 0) merge(1, pre, n_pre);
+  if (prefix) merge(1, pre, n_pre);
   if (wrong) return;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   uint4 o;
@@ -223,6 +228,8 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     w.min_tok = all_narrow ? 1 : narrow_tok + 1;
     w.max_tok = all_narrow ? 0 : INT32_MAX;
     w.prefix_here = prefix && !narrow_prefix;
+    w.fat_tok = !all_narrow && w.prefix_here ? a.tile_tok : 0;
+    w.unit_cost = kWideUnitCost;
     s = launch_pdl(attention_paged_wide_kernel<D>, dim3((unsigned)dev.num_sms), dim3(kThreads),
                    WideSmem<D>::kAlloc, stream, "paged attention launch", tmQ, tmK, tmV, w);
     if (s != HXB_OK) return s;

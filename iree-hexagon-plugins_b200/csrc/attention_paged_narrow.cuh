@@ -235,12 +235,12 @@ __global__ void __launch_bounds__(kNarThreads, 2)
     Ring<kSlots> ring;
     walk([&](int which, const Item& item, int j) -> bool {
       // (the block id is on its way while the slot is waited for)
-      const int blk = item.j0 + j;
-      const int id = loader.block_of(args, item.keys, item_table(args, item), blk);
+      const BlockOf at = block_at(args, item, item.j0 + j);
+      const int id = loader.block_of(args, at.keys, at.table, at.j);
       const int slot = ring.slot();
       if (!__all_sync(0xffffffffu, wait_bar(&kv_empty[slot], ring.parity() ^ 1, fs))) return false;
       loader.load(args, item.head, which ? &tmV : &tmK, smem + L::kOffKV + slot * kTileBytes,
-                  &kv_full[slot], blk, id);
+                  &kv_full[slot], at.j, id);
       ++ring.n;
       return true;
     });
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kNarThreads, 2)
         } else {
           ok = wait_bar(&kv_full[slot], ring.parity(), fs);
           // the key threads zero the rows behind the last one
-          if (ok && last && tail_rows(item) < kBN) {
+          if (ok && last && block_rows_at(args, item, item.j0 + j) < kBN) {
             *v_slot = slot;
             mbar_arrive(v_need);
           }
@@ -475,12 +475,13 @@ __global__ void __launch_bounds__(kNarThreads, 2)
               __float2half_rn(pv);
         }
         ++blocks_done;
-        if (j == blocks - 1 && tail_rows(item) < kBN) {
+        const int live = keys - (key00 + j * kBN);
+        if (live < kBN) {
           // zeros behind the last V row, once the tile has landed
           wait(v_need, fixes++ & 1);
           if (!bad) {
             uint8_t* tile = smem + L::kOffKV + *v_slot * kTileBytes;
-            for (int i = max(tail_rows(item), 0) * 8 + kl; i < kBN * 8; i += 128)
+            for (int i = live * 8 + kl; i < kBN * 8; i += 128)
 #pragma unroll
               for (int b = 0; b < L::kBoxes; ++b)
                 *reinterpret_cast<uint4*>(tile + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kNarThreads, 2)
         else if (!direct) args.whole_lse[kind][at0 + kl] = lse;
         if (item.j0 == 0)
           args.info[kind][at0 + kl] =
-              make_int2(item.first + (slot >= 0 ? kNarrowSlot : 0), item.pieces | (kl << 16));
+              make_int2(item.first | kNarrowSlot, item.pieces | (kl << 16));
       }
       release();
     }

@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   float2* ml = reinterpret_cast<float2*>(smem + L::kOffML);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+  volatile int* v_job = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 8);
   auto& share_smem = *reinterpret_cast<ShareSmem<kThreads>*>(smem + L::kOffShare);
 
   const int warp = threadIdx.x >> 5;
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(xsync, 2 * kBM);
     for (int s = 0; s < kItems; ++s) {
       mbar_init(&item_full[s], 1);
-      mbar_init(&item_empty[s], 3 + 8);  // producer, issuer, tail warp, 8 softmax warps
+      mbar_init(&item_empty[s], 2 + 8);  // producer, issuer, 8 softmax warps
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -149,17 +150,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       Item item;
       while (ok && next_item(item)) {
         if (item.blocks == 0) continue;
-        const int* table = item_table(args, item);
         const bool pair = item.ntok > args.tile_tok;
         const int la = pair ? 1 : 2;  // K blocks ahead of the V block
         auto load_tile = [&](const CUtensorMap* map, int j) -> bool {
           // (the block id is on its way while the slot is waited for)
-          const int block = loader.block_of(args, item.keys, table, item.j0 + j);
+          const BlockOf at = block_at(args, item, item.j0 + j);
+          const int block = loader.block_of(args, at.keys, at.table, at.j);
           const int slot = ring.slot();
           if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[slot], ring.parity() ^ 1, fs)))
             return false;
           loader.load(args, item.head, map, smem + L::kOffKV + slot * kTileBytes, &kv_full[slot],
-                      item.j0 + j, block);
+                      at.j, block);
           ++ring.n;
           return true;
         };
@@ -217,7 +218,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = mbar_wait(q_full, q_items & 1, fs);
           const bool pair = item.ntok > args.tile_tok;
           const int nb = item.blocks;
-          const bool tail = tail_rows(item) < kBN;
           auto wait_tile = [&]() -> bool {
             const bool r = mbar_wait(&kv_full[ring.slot()], ring.parity(), fs);
             tc_fence_after();
@@ -265,8 +265,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int vslot = ring.slot();
             if (!(ok = wait_tile())) break;
             ++ring.n;
-            const bool fix = tail && j == nb - 1;
-            if (fix) mbar_arrive(v_need);  // (zeroed while the softmax runs)
+            const int rows = block_rows_at(args, item, item.j0 + j);
+            const bool fix = rows < kBN;
+            if (fix) {  // (zeroed while the softmax runs)
+              *v_job = vslot << 8 | rows;
+              mbar_arrive(v_need);
+            }
             // both warpgroups have read the previous item's accumulators
             if (j == 0 && q_items && !(ok = mbar_wait(o_free, (q_items & 1) ^ 1, fs))) break;
             const bool more = j + la < nb;
@@ -303,6 +307,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++q_items;
         ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       }
+      if (lane == 0) {
+        *v_job = -1;
+        mbar_arrive(v_need);
+      }
       if (lane == 0 && issued_any) {
         // (complete already on the normal path)
         umma_commit(drain);
@@ -313,20 +321,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 2) {
       // ---------------------------------------- zeros behind the last V row
       // The issuer asks for each such tile when it has landed and waits for
-      // the answer before its PV, so both barriers keep in step.
-      Ring<kSlots> ring;
+      // the answer before its PV, so both barriers keep in step; a job of -1
+      // is the end.
       uint32_t fixes = 0;
-      bool ok = true;
-      Item item;
-      while (ok && next_item(item)) {
-        ring.n += 2 * item.blocks;
-        const int rows = tail_rows(item);
-        if (item.blocks == 0 || rows >= kBN) continue;
-        ok = __all_sync(0xffffffffu, mbar_wait(v_need, fixes++ & 1, fs));
-        if (!ok) break;
-        // the last tile of an item is the V tile of its last block
-        uint8_t* tile = smem + L::kOffKV + (ring.n - 1) % kSlots * kTileBytes;
-        for (int i = max(rows, 0) * 8 + lane; i < kBN * 8; i += 32)
+      while (__all_sync(0xffffffffu, mbar_wait(v_need, fixes++ & 1, fs))) {
+        const int job = *v_job;
+        if (job < 0) break;
+        uint8_t* tile = smem + L::kOffKV + (job >> 8) * kTileBytes;
+        for (int i = (job & 255) * 8 + lane; i < kBN * 8; i += 32)
 #pragma unroll
           for (int b = 0; b < L::kBoxes; ++b)
             *reinterpret_cast<uint4*>(tile + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
@@ -385,12 +387,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; ++e) s[ch * 32 + e] = __uint_as_float(u[e]);
           }
           tmem_wait_ld();
-          const int key0 = (item.j0 + j) * kBN;
-          if (key0 + kBN - 1 > min(item.keys - 1, item.pos0)) {  // not all rows see all keys
-            const int lim = min(item.keys - 1, item.pos0 + token());  // last key this row sees
+          // keys of the block that all rows see, and (fewer) that this row sees
+          const int jj = item.j0 + j - item.pre;
+          int all = jj < 0 ? args.prefix_len - (jj + item.pre) * kBN
+                           : min(item.keys - 1, item.pos0) + 1 - jj * kBN;
+          if (all < kBN) {
+            if (jj >= 0) all = min(item.keys - 1, item.pos0 + token()) + 1 - jj * kBN;
 #pragma unroll
             for (int e = 0; e < kBN; ++e)
-              if (key0 + e > lim) s[e] = -INFINITY;
+              if (e >= all) s[e] = -INFINITY;
           }
           float m8[8];
 #pragma unroll
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const int kind = item.request < 0;
       const int slot = item.slot;
-      const bool direct = slot < 0 && args.prefix_len == 0;
+      const bool direct = slot < 0 && (args.prefix_len == 0 || item.pre > 0);
       const int prow = (pair ? t * kBM : 0) + r;
       const int R = args.total_q * args.group;
       const int pr = (item.tok0 + tok) * args.group + r % args.group;
@@ -508,7 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (pair || t == 0) {
           if (slot >= 0) args.cut_lse[0][slot * 256 + prow] = lse;
           else if (!direct) args.whole_lse[kind][at] = lse;
-          if (item.j0 == 0) args.info[kind][at] = make_int2(item.first, item.pieces | (prow << 16));
+          if (item.j0 == 0)
+            args.info[kind][at] = make_int2(item.first | (item.pre > 0 ? kWithPrefix : 0),
+                                            item.pieces | (prow << 16));
         }
       }
       __half* orow = args.O + ((long long)item.tok0 + tok) * args.ldo +

@@ -4,8 +4,11 @@
 //
 // Work: a "segment" is one key set (the shared prefix, or the own keys of one
 // request), its tokens cut into row units of unit_tok tokens. For every KV head
-// and row unit it visits key blocks of 128. All of that is laid end to end in
-// units of one block -- prefix, request 0, request 1 ...; inside a segment KV
+// and row unit it visits key blocks of 128. Where every request fills tiles by
+// itself (prompt chunks), sharing the prefix would only add partial results: then
+// each request's segment visits the prefix blocks first and its own after them.
+// All of that is laid end to end in units of one block (a row unit counts
+// unit_cost more for its start and end) -- prefix, request 0, request 1 ...; inside a segment KV
 // head by KV head, row unit by row unit -- and CTA i takes units [i S, (i + 1) S),
 // S = ceil(T / CTAs): equal shares whatever the lengths, which are read on the
 // GPU. The part of a row unit's blocks that falls to one CTA is an item;
@@ -29,6 +32,7 @@ constexpr int kEnd = -2;
 // One piece of work: `blocks` key blocks from block j0 of a row unit.
 struct Item {
   int request;  // -1: the shared prefix; kEnd: no more work
+  int pre;      // the first `pre` blocks of the row unit are the prefix's
   int head;     // KV head
   int tok0;     // first token of the row unit
   int ntok;     // its tokens
@@ -36,7 +40,7 @@ struct Item {
   int keys;     // keys of the segment's key set
   int pos0;     // last key that token tok0 sees (causal), else INT_MAX / 2
   int slot;     // partial slot of a cut row unit, -1: it is whole here
-  int first, pieces;  // a cut row unit: slot of its first piece, and how many
+  int first, pieces;  // a cut row unit: CTA of its first piece, and how many
 };
 static_assert(sizeof(Item) <= 64, "item record");
 
@@ -50,8 +54,10 @@ struct PagedArgs {
   long long ldq, ldo, table_ld;
   int total_q, batch, q_heads, kv_heads, group;
   int unit_tok;            // tokens per row unit
+  int unit_cost;           // blocks that its start and end cost
   int min_tok, max_tok;    // this kernel takes the requests of that many tokens
   int prefix_here;         // and the prefix
+  int fat_tok;             // requests of so many tokens fill tiles (0: no matter)
   int tile_tok, box_tok;   // wide kernel: tokens per 128-row tile and per Q box
   int table_cols, num_blocks, rows_log2;
   int prefix_len;
@@ -61,13 +67,13 @@ struct PagedArgs {
   // pr = token * group + head-in-group of KV head h. Four columns of a row lie
   // together and the rows of a tile side by side, so that threads that hold a
   // row each write and read whole lines:
-  //   cut row units  cut_o[kernel][slot][D / 4][rows][4], slot = 2 CTA (the
-  //                  CTA's first item) or 2 CTA + 1 (its last); rows = 256
+  //   cut row units  cut_o[kernel][slot][D / 4][rows][4], slot = 2 CTA + 1 for
+  //                  the unit's first piece, 2 CTA for the others; rows = 256
   //                  (wide, kernel 0) or 16 (narrow, kernel 1)
   //   whole ones     whole_o[set][h][D / 4][total_q * group][4], set = 0 own
   //                  keys, 1 prefix
-  // info[set][h][pr]: {slot of the first piece (narrow: + kNarrowSlot),
-  // pieces | row in the slot << 16}
+  // info[set][h][pr]: {CTA of the first piece | flags, pieces | row in the slot
+  // << 16}
   float* cut_o[2];
   float* cut_lse[2];
   float* whole_o[2];
@@ -76,7 +82,8 @@ struct PagedArgs {
   int ctas[2];
   int* status;
 };
-constexpr int kNarrowSlot = 1 << 30;
+constexpr int kNarrowSlot = 1 << 30;  // flag: the narrow kernel's slots
+constexpr int kWithPrefix = 1 << 29;  // flag: the prefix is in these pieces
 
 // Position in a ring of N slots, counted in uses.
 template <int N>
@@ -105,7 +112,8 @@ __device__ __forceinline__ int clamp_token(const PagedArgs& a, int b) {
 struct Segment {
   int tok, n, keys;
   int units;       // row units
-  int work;        // blocks of one KV head over all row units
+  int work;        // units of work of one KV head over all row units
+  int pre;         // prefix blocks visited before the own ones
   bool causal;
 };
 
@@ -117,7 +125,8 @@ __device__ __forceinline__ int unit_keys(const PagedArgs& a, const Segment& s, i
 }
 
 __device__ __forceinline__ int unit_blocks(const PagedArgs& a, const Segment& s, int u) {
-  return max(1, (unit_keys(a, s, u) + kBN - 1) / kBN);  // an empty unit still writes its rows
+  // (a unit without keys still writes its rows)
+  return max(1, s.pre + (unit_keys(a, s, u) + kBN - 1) / kBN);
 }
 
 // sum_{i < n} floor((a i + b) / m), by the Euclidean algorithm on (a, m): whole
@@ -141,45 +150,56 @@ __device__ __forceinline__ long long floor_sum(unsigned n, unsigned m, unsigned 
 
 constexpr int kMostWork = 1 << 30;  // blocks of one call (saturated above)
 
-// Blocks of the first `units` row units of one KV head.
-__device__ __forceinline__ int blocks_before(const PagedArgs& a, const Segment& s, int units) {
-  if (units <= 1) return units == 0 ? 0 : unit_blocks(a, s, 0);
-  if (!s.causal) return (int)min((long long)units * unit_blocks(a, s, 0), (long long)kMostWork);
-  // unit u < units - 1 sees d + (u + 1) T keys: none up to u = dark (one block
-  // each), then one block per begun 128
-  const int T = a.unit_tok, d = s.keys - s.n, full = units - 1;
-  const int dark = d < 0 ? min(full, (-d) / T) : 0;
-  long long sum = dark;
-  if (full > dark) sum += floor_sum(full - dark, kBN, T, d + (dark + 1) * T + kBN - 1);
-  return (int)min(sum + unit_blocks(a, s, full), (long long)kMostWork);
+// Work of the first `units` row units of one KV head.
+__device__ __forceinline__ int work_before(const PagedArgs& a, const Segment& s, int units) {
+  long long sum = (long long)units * a.unit_cost;
+  if (units <= 1 || !s.causal) {
+    if (units) sum += (long long)units * unit_blocks(a, s, 0);
+  } else {
+    // unit u < units - 1 sees d + (u + 1) T own keys: none up to u = dark, then
+    // one block per begun 128
+    const int T = a.unit_tok, d = s.keys - s.n, full = units - 1;
+    const int dark = d < 0 ? min(full, (-d) / T) : 0;
+    sum += (long long)dark * max(1, s.pre) + (long long)(full - dark) * s.pre;
+    if (full > dark) sum += floor_sum(full - dark, kBN, T, d + (dark + 1) * T + kBN - 1);
+    sum += unit_blocks(a, s, full);
+  }
+  return (int)min(sum, (long long)kMostWork);
 }
 
-__device__ __forceinline__ Segment own_segment(const PagedArgs& a, int b) {
+__device__ __forceinline__ int own_tokens(const PagedArgs& a, int b) {
+  return max(clamp_token(a, b + 1) - clamp_token(a, b), 0);
+}
+
+__device__ __forceinline__ Segment own_segment(const PagedArgs& a, int b, int pre) {
   Segment s;
   s.tok = clamp_token(a, b);
-  s.n = max(clamp_token(a, b + 1) - s.tok, 0);
+  s.n = own_tokens(a, b);
   if (s.n < a.min_tok || s.n > a.max_tok) s.n = 0;  // the other kernel's
   s.keys = (int)min((long long)max(a.kv_lens[b], 0), (long long)a.table_cols << a.rows_log2);
   s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
+  s.pre = pre;
   s.causal = a.causal != 0;
-  s.work = s.units ? blocks_before(a, s, s.units) : 0;
+  s.work = work_before(a, s, s.units);
   return s;
 }
 
-__device__ __forceinline__ Segment prefix_segment(const PagedArgs& a) {
+__device__ __forceinline__ Segment prefix_segment(const PagedArgs& a, bool here) {
   Segment s;
   s.tok = clamp_token(a, 0);
-  s.n = a.prefix_here ? max(clamp_token(a, a.batch) - s.tok, 0) : 0;
+  s.n = here ? max(clamp_token(a, a.batch) - s.tok, 0) : 0;
   s.keys = a.prefix_len;
   s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
+  s.pre = 0;
   s.causal = false;
-  s.work = (int)min((long long)s.units * ((s.keys + kBN - 1) / kBN), (long long)kMostWork);
+  s.work = work_before(a, s, s.units);
   return s;
 }
 
 // A CTA's share of the work: units [lo, hi), `per` units per CTA.
 struct Share {
   int lo, hi, per;
+  int pre;  // prefix blocks of the requests' own segments
 };
 template <int THREADS>
 struct ShareSmem {
@@ -194,14 +214,26 @@ struct ShareSmem {
 template <int THREADS>
 __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREADS>& sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Segment pre = prefix_segment(a);
   const int each = a.min_tok <= a.max_tok ? (a.batch + THREADS - 1) / THREADS : 0;
   const int b0 = min((int)threadIdx.x * each, a.batch), b1 = min(b0 + each, a.batch);
+  // every request fills tiles by itself: no shared pass over the prefix
+  bool fat = false;
+  if (a.fat_tok) {
+    bool thin = false;
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+      const int n = own_tokens(a, b);
+      thin |= n > 0 && n < a.fat_tok;
+    }
+    fat = !__syncthreads_or(thin);
+  }
+  Share r{0, 0, 1, fat ? (a.prefix_len + kBN - 1) / kBN : 0};
+  const Segment pre = prefix_segment(a, a.prefix_here && !fat);
   long long mine = 0;
   Segment s;
 #pragma unroll 1
   for (int b = b0; b < b1; ++b) {
-    s = own_segment(a, b);
+    s = own_segment(a, b, r.pre);
     mine += (long long)s.work * a.kv_heads;
   }
   long long scan = mine;
@@ -220,7 +252,6 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
     total += sm.sum[w];
   }
   base += scan - mine;
-  Share r{0, 0, 1};
   if (total >= kMostWork) {  // (hours of work: not started)
     if (threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
     return r;
@@ -233,7 +264,7 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
       int at = (int)base;
 #pragma unroll 1
       for (int b = b0; b < b1; ++b) {
-        if (each > 1) s = own_segment(a, b);
+        if (each > 1) s = own_segment(a, b, r.pre);
         const int w = s.work * a.kv_heads;
         if (r.lo < at + w) {
           sm.b = b;
@@ -274,7 +305,7 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
                                          uint64_t* item_full, uint64_t* item_empty,
                                          const FailState& fs) {
   Ring<N> out;
-  int b = -1, h = 0, u = 0, j = 0;
+  int b = -1, h = 0, u = 0, at = 0;  // next: unit of work `at` of row unit u
   int pos = sh.lo;
   Segment s;
   s.work = 0;
@@ -285,56 +316,54 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
   if (sh.lo < sh.hi) {
     s = sm.seg;
     b = sm.b;
-    int off = max(sm.off, 0);
+    at = max(sm.off, 0);
     if (s.work > 0) {
-      h = min(off / s.work, a.kv_heads);
-      off = min(off - h * s.work, s.work - 1);
-      int above = s.units;  // blocks_before(u) <= off < blocks_before(above)
+      h = min(at / s.work, a.kv_heads);
+      at = min(at - h * s.work, s.work - 1);
+      int above = s.units;  // work_before(u) <= at < work_before(above)
       while (above - u > 1) {
         const int mid = (u + above) >> 1;
-        if (blocks_before(a, s, mid) <= off) u = mid;
+        if (work_before(a, s, mid) <= at) u = mid;
         else above = mid;
       }
-      if (u) off -= blocks_before(a, s, u);
-      j = off;
+      if (u) at -= work_before(a, s, u);
     }
   }
+  const int cost = a.unit_cost;
 #pragma unroll 1
   while (true) {
     Item item;
     item.request = kEnd;
     item.blocks = 0;
     const int kb = unit_blocks(a, s, u);
-    if (pos < sh.hi && s.work > 0 && h < a.kv_heads && u < s.units && j < kb) {
-      const int take = min(kb - j, sh.hi - pos);
+    if (pos < sh.hi && s.work > 0 && h < a.kv_heads && u < s.units && at < kb + cost) {
+      const int take = min(kb + cost - at, sh.hi - pos);
+      const int begin = pos - at + cost;  // its first block, as a unit of work
+      const int j = max(at - cost, 0), blocks = at + take - cost - j;
+      const int keys = unit_keys(a, s, u);
       item.request = b;
+      item.pre = s.pre;
       item.head = h;
       item.tok0 = s.tok + u * a.unit_tok;
       item.ntok = min(s.n - u * a.unit_tok, a.unit_tok);
       item.j0 = j;
       item.keys = s.keys;
       item.pos0 = s.causal ? s.keys - s.n + u * a.unit_tok : INT32_MAX / 2;
-      const bool empty = s.keys == 0 || item.pos0 + item.ntok <= 0;
-      item.blocks = empty ? 0 : take;
-      item.slot = -1;
-      item.pieces = 1;
-      item.first = 0;
-      if (j != 0 || take != kb) {
-        const int begin = pos - j, c0 = begin / sh.per;
-        item.first = 2 * c0 + (c0 * sh.per != begin);
-        item.pieces = (begin + kb - 1) / sh.per - c0 + 1;
-        item.slot = 2 * (int)blockIdx.x + (pos != sh.lo);
-      }
+      item.blocks = keys + s.pre > 0 ? blocks : 0;
+      item.first = begin / sh.per;
+      item.pieces = (begin + kb - 1) / sh.per - item.first + 1;
+      item.slot = item.pieces > 1 ? 2 * (int)blockIdx.x + (j == 0) : -1;
       pos += take;
-      j = 0;
+      at = 0;
       if (pos < sh.hi && ++u == s.units) {
         u = 0;
         if (++h == a.kv_heads) {
           h = 0;
           s.work = 0;
-          while (s.work == 0 && b + 1 < a.batch) s = own_segment(a, ++b);
+          while (s.work == 0 && b + 1 < a.batch) s = own_segment(a, ++b, sh.pre);
         }
       }
+      if (blocks <= 0) continue;  // only the start of a row unit: the next CTA's
     }
     uint64_t* free_slot = &item_empty[out.slot()];
     const uint32_t parity = out.parity() ^ 1;
@@ -380,14 +409,22 @@ struct TileLoader {
   }
 };
 
-// Block table of an item.
-__device__ __forceinline__ const int* item_table(const PagedArgs& a, const Item& item) {
-  return item.request < 0 ? a.prefix_table : a.block_table + (long long)item.request * a.table_ld;
+// Where block j of an item's row unit lies: block `j` of the key set with `keys`
+// keys behind `table`.
+struct BlockOf {
+  const int* table;
+  int keys, j;
+};
+template <typename I>
+__device__ __forceinline__ BlockOf block_at(const PagedArgs& a, const I& item, int j) {
+  if (j < item.pre || item.request < 0) return {a.prefix_table, a.prefix_len, j};
+  return {a.block_table + (long long)item.request * a.table_ld, item.keys, j - item.pre};
 }
-// Rows of the item's last key block that exist; a block with fewer than 128 gets
-// the others of its V tile zeroed (their P is 0, but 0 * NaN is not).
-__device__ __forceinline__ int tail_rows(const Item& item) {
-  return item.keys - (item.j0 + item.blocks - 1) * kBN;
+// Rows of block j that exist; a block with fewer than 128 gets the others of its
+// V tile zeroed (their P is 0, but 0 * NaN is not).
+template <typename I>
+__device__ __forceinline__ int block_rows_at(const PagedArgs& a, const I& item, int j) {
+  return j < item.pre ? a.prefix_len - j * kBN : item.keys - (j - item.pre) * kBN;
 }
 
 }  // namespace hxb

@@ -151,6 +151,12 @@ class Batch:
     ([1] * 17, [40 * i for i in range(17)], 8, 1, 128, 16, 0, True),      # no prefix, ragged
     ([1] * 600, [(i * 7) % 40 for i in range(600)], 4, 2, 64, 16, 70, True),  # many requests
     ([1] * 2, [3000, 17], 32, 8, 128, 16, 4000, True),     # cut across many CTAs
+    # every request fills tiles by itself: each visits the prefix before its own keys
+    ([200, 150], [200, 300], 8, 2, 128, 16, 300, True),
+    ([64, 100, 0, 33], [64, 10, 9, 700], 32, 8, 128, 128, 129, True),
+    ([700], [900], 16, 2, 64, 32, 1000, True),
+    ([150, 140], [0, 333], 9, 3, 64, 16, 77, True),
+    ([130, 257], [300, 20], 4, 4, 128, 64, 128, False),
 ])
 def test_attention_paged_vs_float64(cuda_pkg, new, lens, Hq, Hkv, D, P, prefix, causal):
     Batch(new, lens, Hq, Hkv, D, P, prefix, seed=sum(lens) + prefix).check(
