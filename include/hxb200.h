@@ -518,33 +518,46 @@ hxb_status_t hxb_kv_cache_write_paged_f16(const void* k_src, const void* v_src,
 
 /* Grouped-query attention of a batch over a paged cache, behind a prefix that
  * all its requests share and that is read once for all of them. Rows
- * [q_start[b], q_start[b + 1]) of Q and O are the tokens of request b; they
+ * [q_start[b], q_start[b + 1]) of q and out are the tokens of request b; they
  * attend to
  *   - the prefix_len rows of the prefix's blocks (prefix_table, all visible),
  *   - the first kv_lens[b] rows of the request's own blocks (block_table);
  *     causal != 0 hides own row j > kv_lens[b] - n + i from token i of n (the
  *     tokens are the last cached rows).
- *   Q, O  [total_q, q_heads, head_dim] f16, rows ldq / ldo elements apart
- *         (multiples of 8; Q may be columns of a fused QKV projection)
  * Query head h reads KV head h / (q_heads / kv_heads), at most 128 query heads
  * per KV head; head_dim 64 or 128. prefix_len 0 runs without a prefix. Tokens
- * that see no key are 0; rows of O before q_start[0] and from
+ * that see no key are 0; rows of out before q_start[0] and from
  * q_start[batch] on are left as they are. Cache rows behind a length are not
  * used, whatever they hold; rows within it must be finite where a token of
  * the request may not see them. f32 scores, statistics and sums; P is rounded
- * to f16 for the second product.
- * max_q_len: the most tokens a request is expected to have (1 for decode).
- * Requests may have more; it chooses kernels, not results. workspace:
- * hxb_attention_paged_workspace_bytes(...) bytes, 16-byte aligned, no initial
- * contents; calls that share one must be ordered (one stream). */
-hxb_status_t hxb_attention_paged_f16(
-    const void* Q, int64_t ldq, void* O, int64_t ldo, const int32_t* q_start,
-    const int32_t* kv_lens, int64_t batch, int64_t total_q, int64_t max_q_len,
-    const void* k_cache, const void* v_cache, int64_t block_stride, int64_t num_blocks,
-    int64_t block_rows, const int32_t* block_table, int64_t table_ld, int64_t table_cols,
-    const int32_t* prefix_table, int64_t prefix_len, int64_t q_heads, int64_t kv_heads,
-    int64_t head_dim, float scale, int causal, void* workspace, size_t workspace_bytes,
-    void* stream);
+ * to f16 for the second product. A call of more than 2^30 pairs of a query
+ * tile and a key block is not run (HXB_DEVICE_STATUS_BAD_INDEX). */
+typedef struct hxb_attention_paged_s {
+  const void* q;            /* f16 [total_q, q_heads, head_dim], rows ldq apart */
+  int64_t ldq;              /* (elements, a multiple of 8; q may be columns of */
+  void* out;                /* a fused QKV projection); out alike */
+  int64_t ldo;
+  const int32_t* q_start;   /* [batch + 1] */
+  const int32_t* kv_lens;   /* [batch] */
+  int64_t batch, total_q;
+  int64_t max_q_len;        /* the most tokens a request is expected to have (1 */
+                            /* for decode): chooses kernels, not results */
+  const void* k_cache;
+  const void* v_cache;
+  int64_t block_stride, num_blocks, block_rows;
+  const int32_t* block_table;
+  int64_t table_ld, table_cols;
+  const int32_t* prefix_table;
+  int64_t prefix_len;
+  int64_t q_heads, kv_heads, head_dim;
+  float scale;              /* finite, > 0 */
+  int32_t causal;
+  void* workspace;          /* hxb_attention_paged_workspace_bytes, 16-byte */
+  uint64_t workspace_bytes; /* aligned, no initial contents; calls that share */
+                            /* one must be ordered (one stream) */
+} hxb_attention_paged_t;
+
+hxb_status_t hxb_attention_paged_f16(const hxb_attention_paged_t* args, void* stream);
 
 /* Workspace of hxb_attention_paged_f16 on the current device (0 if the extents
  * are invalid or total_q is 0). */

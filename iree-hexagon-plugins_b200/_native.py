@@ -79,10 +79,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                  c_vp, c_vp, c_vp, c_i64, c_vp, c_vp]),
     "hxb_kv_cache_write_paged_f16": (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
                                              c_i64, c_i64, c_i64, c_i64, c_vp]),
-    "hxb_attention_paged_f16": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64,
-                                        c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp,
-                                        c_i64, c_i64, c_i64, c_i64, c_float, c_int, c_vp, c_size,
-                                        c_vp]),
+    "hxb_attention_paged_f16": (c_int, [c_vp, c_vp]),
     "hxb_attention_paged_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
     # include/hxb200_hal.h: executable library
     "hxb_executable_library_query": (c_vp, [ctypes.c_uint32, c_vp]),
@@ -278,6 +275,20 @@ class DecoderW8(ctypes.Structure):
                 ("w_o", c_vp), ("s_o", c_vp), ("ffn_norm", c_vp),
                 ("w_gate_up", c_vp), ("s_gate_up", c_vp),
                 ("w_down", c_vp), ("s_down", c_vp)]
+
+
+class AttentionPaged(ctypes.Structure):
+    """hxb_attention_paged_t of include/hxb200.h."""
+
+    _fields_ = [("q", c_vp), ("ldq", c_i64), ("out", c_vp), ("ldo", c_i64),
+                ("q_start", c_vp), ("kv_lens", c_vp), ("batch", c_i64), ("total_q", c_i64),
+                ("max_q_len", c_i64), ("k_cache", c_vp), ("v_cache", c_vp),
+                ("block_stride", c_i64), ("num_blocks", c_i64), ("block_rows", c_i64),
+                ("block_table", c_vp), ("table_ld", c_i64), ("table_cols", c_i64),
+                ("prefix_table", c_vp), ("prefix_len", c_i64), ("q_heads", c_i64),
+                ("kv_heads", c_i64), ("head_dim", c_i64), ("scale", c_float),
+                ("causal", ctypes.c_int32), ("workspace", c_vp), ("workspace_bytes", c_u64)]
+
 
 STATUS_NAMES = {
     0: "OK",

@@ -273,15 +273,13 @@ extern "C" size_t hxb_attention_paged_workspace_bytes(int64_t total_q, int64_t q
   return paged_layout(total_q * q_heads, head_dim, prefix_len > 0, dev->num_sms).total;
 }
 
-extern "C" hxb_status_t hxb_attention_paged_f16(
-    const void* Q, int64_t ldq, void* O, int64_t ldo, const int32_t* q_start,
-    const int32_t* kv_lens, int64_t batch, int64_t total_q, int64_t max_q_len,
-    const void* k_cache, const void* v_cache, int64_t block_stride, int64_t num_blocks,
-    int64_t block_rows, const int32_t* block_table, int64_t table_ld, int64_t table_cols,
-    const int32_t* prefix_table, int64_t prefix_len, int64_t q_heads, int64_t kv_heads,
-    int64_t head_dim, float scale, int causal, void* workspace, size_t workspace_bytes,
-    void* stream) {
+extern "C" hxb_status_t hxb_attention_paged_f16(const hxb_attention_paged_t* args, void* stream) {
   using namespace hxb;
+  if (!args) return fail(HXB_STATUS_INVALID_ARGUMENT, "paged attention: null arguments");
+  const auto& [Q, ldq, O, ldo, q_start, kv_lens, batch, total_q, max_q_len, k_cache, v_cache,
+               block_stride, num_blocks, block_rows, block_table, table_ld, table_cols,
+               prefix_table, prefix_len, q_heads, kv_heads, head_dim, scale, causal, workspace,
+               workspace_bytes] = *args;
   if (head_dim != 64 && head_dim != 128)
     return fail(HXB_STATUS_UNSUPPORTED, "paged attention: head dim %lld not supported (64 or 128)",
                 (long long)head_dim);

@@ -17,56 +17,63 @@ batch (integration_tests/models/kv_cache.py:91-112).
 from __future__ import annotations
 
 import contextlib
+import functools
+import struct
 
 import torch
 
 from . import _native
 from ._native import check
-from .dispatch import _require
 
+# hxb_attention_paged_t: packing the record is several times cheaper than
+# converting its 26 fields one by one.
+_ARGUMENTS = struct.Struct("=QqQqQQqqqQQqqqQqqQqqqqfiQQ")
 _NO_GUARD = contextlib.nullcontext()
+_I32, _I64, _F16 = torch.int32, torch.int64, torch.float16
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _on(device: torch.device):
     """A guard that makes `device` current for a call (nothing to do on it)."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index == torch.cuda.current_device():
         return _NO_GUARD
     return torch.cuda.device(device)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, numel: int, device: torch.device) -> int:
+def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, numel: int, index: int) -> int:
     """Data pointer of a contiguous integer tensor of at least `numel` elements."""
-    if t.dtype != dtype or t.device != device or t.numel() < numel or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != index or t.numel() < numel or \
+            not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of at least {numel} elements "
-                         f"on {device}")
+                         f"on cuda:{index}")
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, device: torch.device) -> tuple[int, int, int]:
+def _table(t: torch.Tensor, rows: int, index: int) -> tuple[int, int, int]:
     """(pointer, row pitch, columns) of a block table."""
-    if t.dim() != 2 or t.dtype != torch.int32 or t.device != device or \
-            (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"block_table must be a 2-D int32 tensor with unit inner stride on {device}")
+    if t.dim() != 2 or t.dtype is not _I32 or t.get_device() != index or t.shape[0] != rows or \
+            (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"block_table must be a 2-D int32 tensor with one row per request ({rows}) and "
+                         f"unit inner stride on cuda:{index}")
     cols = t.shape[1]
-    return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else cols), cols
+    return t.data_ptr(), (t.stride(0) if rows > 1 else cols), cols
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int, int]:
-    """(blocks, KV heads, rows per block, head dim, block stride) of a cache."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or \
-            k_cache.dtype != torch.float16 or v_cache.dtype != torch.float16:
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int, int, int, int]:
+    """(device index, blocks, KV heads, rows per block, head dim, block stride)
+    of a cache."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype is not _F16 or \
+            v_cache.dtype is not _F16:
         raise ValueError("k_cache / v_cache must be f16 [blocks, kv_heads, block_rows, head_dim]")
-    n, h, p, d = k_cache.shape
+    n, h, p, d = shape
     stride = k_cache.stride()
     if v_cache.stride() != stride or stride[1:] != (p * d, d, 1):
         raise ValueError("the blocks of k_cache / v_cache must be contiguous, with one stride")
-    _require(k_cache.is_cuda and v_cache.device == k_cache.device,
-             "k_cache / v_cache must be on one CUDA device")
-    return n, h, p, d, (stride[0] if n > 1 else h * p * d)
+    index = k_cache.get_device()
+    if index < 0 or v_cache.get_device() != index:
+        raise ValueError("k_cache / v_cache must be on one CUDA device")
+    return index, n, h, p, d, (stride[0] if n > 1 else h * p * d)
 
 
 def paged_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks: torch.Tensor,
@@ -84,33 +91,33 @@ def paged_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks:
     and `cursor_out` may be `cursor` (of 2 elements). `max_tokens` is needed
     unless `slots` is given, whose length it then is."""
     lib = _native.load()
-    dev = cached_lens.device
-    _require(cached_lens.is_cuda, "cached_lens must be a CUDA tensor")
+    index = cached_lens.get_device()
+    if index < 0 or block_rows < 1:
+        raise ValueError("cached_lens must be a CUDA tensor and block_rows >= 1")
     B = cached_lens.numel()
-    i32 = torch.int32
-    cached_p = _ints("cached_lens", cached_lens, i32, B, dev)
-    new_p = _ints("new_lens", new_lens, i32, B, dev)
-    free_p = _ints("free_blocks", free_blocks, i32, 0, dev)
-    cursor_p = _ints("cursor", cursor, i32, 1, dev)
-    table_p, ld, cols = _table(block_table, dev)
-    _require(block_table.shape[0] == B, "block_table must have one row per request")
-    _require(new_lens.numel() == B, "cached_lens and new_lens must have one entry per request")
+    if new_lens.numel() != B:
+        raise ValueError("cached_lens and new_lens must have one entry per request")
     if slots is None:
-        _require(max_tokens is not None, "max_tokens or slots is needed")
-        slots = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+        if max_tokens is None:
+            raise ValueError("max_tokens or slots is needed")
+        slots = cached_lens.new_empty(max_tokens, dtype=_I64)
     n = slots.numel() if max_tokens is None else int(max_tokens)
     if q_start is None:
-        q_start = torch.empty(B + 1, dtype=i32, device=dev)
+        q_start = cached_lens.new_empty(B + 1)
     if kv_lens is None:
-        kv_lens = torch.empty(B, dtype=i32, device=dev)
+        kv_lens = cached_lens.new_empty(B)
     if cursor_out is None:
-        cursor_out = torch.empty(2, dtype=i32, device=dev)
-    with _on(dev):
+        cursor_out = cached_lens.new_empty(2)
+    table_p, ld, cols = _table(block_table, B, index)
+    with _on(cached_lens.device):
         check(lib.hxb_paged_tables(
-            cached_p, new_p, B, block_rows, free_p, free_blocks.numel(), cursor_p, table_p, ld,
-            cols, _ints("q_start", q_start, i32, B + 1, dev), _ints("kv_lens", kv_lens, i32, B, dev),
-            _ints("slots", slots, torch.int64, n, dev), n,
-            _ints("cursor_out", cursor_out, i32, 2, dev), _stream(dev)))
+            _ints("cached_lens", cached_lens, _I32, B, index),
+            _ints("new_lens", new_lens, _I32, B, index), B, block_rows,
+            _ints("free_blocks", free_blocks, _I32, 0, index), free_blocks.numel(),
+            _ints("cursor", cursor, _I32, 1, index), table_p, ld, cols,
+            _ints("q_start", q_start, _I32, B + 1, index), _ints("kv_lens", kv_lens, _I32, B, index),
+            _ints("slots", slots, _I64, n, index), n,
+            _ints("cursor_out", cursor_out, _I32, 2, index), _raw_stream(index)))
     return q_start, kv_lens, slots, cursor_out
 
 
@@ -121,20 +128,26 @@ def kv_cache_write_paged(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torc
     Sources are [tokens, kv_heads * D] f16 views of one row pitch (e.g. column
     blocks of a fused QKV output), caches [blocks, kv_heads, block_rows, D]."""
     lib = _native.load()
-    blocks, heads, rows, D, stride = _cache(k_cache, v_cache)
-    dev = k_cache.device
-    if k_src.dim() != 2 or k_src.shape != v_src.shape or k_src.stride() != v_src.stride() or \
-            k_src.dtype != torch.float16 or v_src.dtype != torch.float16 or \
-            k_src.shape[1] != heads * D or k_src.stride(1) != 1:
+    index, blocks, heads, rows, D, stride = _cache(k_cache, v_cache)
+    shape, src_stride = k_src.shape, k_src.stride()
+    if len(shape) != 2 or shape[1] != heads * D or shape != v_src.shape or src_stride[1] != 1 or \
+            src_stride != v_src.stride() or k_src.dtype is not _F16 or v_src.dtype is not _F16:
         raise ValueError("k_src / v_src must be f16 [tokens, kv_heads * head_dim] views of one layout "
                          "with unit inner stride")
-    _require(k_src.device == dev and v_src.device == dev, "sources and caches must share a device")
-    n = k_src.shape[0]
-    ld = k_src.stride(0) if n > 1 else heads * D
-    with _on(dev):
+    if k_src.get_device() != index or v_src.get_device() != index:
+        raise ValueError("sources and caches must share a device")
+    n = shape[0]
+    with _on(k_cache.device):
         check(lib.hxb_kv_cache_write_paged_f16(
-            k_src.data_ptr(), v_src.data_ptr(), ld, _ints("slots", slots, torch.int64, n, dev), n,
-            k_cache.data_ptr(), v_cache.data_ptr(), stride, blocks, heads, rows, D, _stream(dev)))
+            k_src.data_ptr(), v_src.data_ptr(), src_stride[0] if n > 1 else heads * D,
+            _ints("slots", slots, _I64, n, index), n, k_cache.data_ptr(), v_cache.data_ptr(), stride,
+            blocks, heads, rows, D, _raw_stream(index)))
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(index: int, total_q: int, q_heads: int, head_dim: int, prefix: bool) -> int:
+    with torch.cuda.device(index):
+        return attention_paged_workspace_bytes(total_q, q_heads, head_dim, int(prefix))
 
 
 def attention_paged_workspace_bytes(total_q: int, q_heads: int, head_dim: int,
@@ -161,41 +174,46 @@ def attention_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     are left as they are. `workspace`: a device buffer of
     attention_paged_workspace_bytes, allocated here if None."""
     lib = _native.load()
-    blocks, Hkv, rows, D, stride = _cache(k_cache, v_cache)
-    dev = k_cache.device
-    if query.dim() != 3 or query.dtype != torch.float16 or query.device != dev or \
-            query.shape[2] != D or query.stride(2) != 1 or query.stride(1) != D:
+    index, blocks, Hkv, rows, D, stride = _cache(k_cache, v_cache)
+    shape, q_stride = query.shape, query.stride()
+    if len(shape) != 3 or shape[2] != D or q_stride[2] != 1 or q_stride[1] != D or \
+            query.dtype is not _F16 or query.get_device() != index:
         raise ValueError("query must be f16 [tokens, q_heads, head_dim] with contiguous heads on the "
                          "caches' device")
-    n, Hq, _ = query.shape
+    n, Hq, _ = shape
     if out is None:
-        out = torch.empty((n, Hq, D), dtype=torch.float16, device=dev)
-    elif out.shape != query.shape or out.dtype != torch.float16 or out.device != dev or \
-            out.stride(2) != 1 or out.stride(1) != D:
-        raise ValueError("out must match query's shape, type and device, with contiguous heads")
+        out = k_cache.new_empty(shape)
+        o_stride = out.stride()
+    else:
+        o_stride = out.stride()
+        if out.shape != shape or o_stride[2] != 1 or o_stride[1] != D or \
+                out.dtype is not _F16 or out.get_device() != index:
+            raise ValueError("out must match query's shape, type and device, with contiguous heads")
+    if n == 0:
+        return out
     B = kv_lens.numel()
-    table_p, ld, cols = _table(block_table, dev)
-    _require(block_table.shape[0] == B, "block_table must have one row per request")
+    table_p, ld, cols = _table(block_table, B, index)
     prefix_len = int(prefix_len)
-    prefix_p = None
-    if prefix_len:
-        _require(prefix_table is not None, "prefix_len needs prefix_table")
-        prefix_p = _ints("prefix_table", prefix_table, torch.int32, -(-prefix_len // rows), dev)
+    prefix_p = 0
+    if prefix_len > 0:
+        if prefix_table is None:
+            raise ValueError("prefix_len needs prefix_table")
+        prefix_p = _ints("prefix_table", prefix_table, _I32, -(-prefix_len // rows), index)
     row = Hq * D
-    with _on(dev):
+    with _on(k_cache.device):
         if workspace is None:
-            workspace = torch.empty(
-                lib.hxb_attention_paged_workspace_bytes(n, Hq, D, prefix_len), dtype=torch.uint8,
-                device=dev)
+            nbytes = _workspace_bytes(index, n, Hq, D, prefix_len > 0)
+            workspace = kv_lens.new_empty(nbytes >> 2)
         else:
-            _require(workspace.device == dev and workspace.is_contiguous(),
-                     "workspace must be a contiguous buffer on the caches' device")
-        check(lib.hxb_attention_paged_f16(
-            query.data_ptr(), query.stride(0) if n > 1 else row, out.data_ptr(),
-            out.stride(0) if n > 1 else row, _ints("q_start", q_start, torch.int32, B + 1, dev),
-            _ints("kv_lens", kv_lens, torch.int32, B, dev), B, n,
+            if workspace.get_device() != index or not workspace.is_contiguous():
+                raise ValueError("workspace must be a contiguous buffer on the caches' device")
+            nbytes = workspace.numel() * workspace.element_size()
+        check(lib.hxb_attention_paged_f16(_ARGUMENTS.pack(
+            query.data_ptr(), q_stride[0] if n > 1 else row, out.data_ptr(),
+            o_stride[0] if n > 1 else row, _ints("q_start", q_start, _I32, B + 1, index),
+            _ints("kv_lens", kv_lens, _I32, B, index), B, n,
             n if max_q_len is None else max_q_len, k_cache.data_ptr(), v_cache.data_ptr(), stride,
             blocks, rows, table_p, ld, cols, prefix_p, prefix_len, Hq, Hkv, D,
-            D ** -0.5 if scale is None else float(scale), int(causal), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _stream(dev)))
+            D ** -0.5 if scale is None else scale, bool(causal), workspace.data_ptr(), nbytes),
+            _raw_stream(index)))
     return out

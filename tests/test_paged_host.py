@@ -2,57 +2,74 @@
 before any device access (no GPU needed; the pointers are never followed)."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 
 A = 0x100000  # an aligned address
 
 
-def attention(lib, **kw):
-    a = dict(Q=A, ldq=1024, O=A, ldo=1024, q_start=A, kv_lens=A, batch=2, total_q=2, max_q=1, k=A, v=A,
-             stride=2 * 16 * 128, blocks=8, rows=16, table=A, table_ld=4, cols=4, ptable=A, prefix=20,
-             q_heads=8, kv_heads=2, D=128, scale=0.1, causal=1, ws=A, ws_bytes=1 << 40, stream=None)
-    assert set(kw) <= set(a)
-    a.update(kw)
-    return lib.hxb_attention_paged_f16(*a.values())
+def attention(pkg, **kw):
+    a = pkg._native.AttentionPaged(
+        q=A, ldq=1024, out=A, ldo=1024, q_start=A, kv_lens=A, batch=2, total_q=2, max_q_len=1, k_cache=A,
+        v_cache=A, block_stride=2 * 16 * 128, num_blocks=8, block_rows=16, block_table=A, table_ld=4,
+        table_cols=4, prefix_table=A, prefix_len=20, q_heads=8, kv_heads=2, head_dim=128, scale=0.1,
+        causal=1, workspace=A, workspace_bytes=1 << 40)
+    for name, value in kw.items():
+        assert hasattr(a, name)
+        setattr(a, name, value)
+    return pkg._native.load().hxb_attention_paged_f16(ctypes.byref(a), None)
 
 
 @pytest.mark.parametrize("kw,status,text", [
-    (dict(D=96), 2, b"head dim 96"),
-    (dict(rows=48), 2, b"power of two"),
-    (dict(rows=8), 2, b"power of two"),
-    (dict(rows=2048, stride=2 * 2048 * 128), 2, b"power of two"),
+    (dict(head_dim=96), 2, b"head dim 96"),
+    (dict(block_rows=48), 2, b"power of two"),
+    (dict(block_rows=8), 2, b"power of two"),
+    (dict(block_rows=2048, block_stride=2 * 2048 * 128), 2, b"power of two"),
     (dict(q_heads=9), 1, b"multiple of kv_heads"),
     (dict(q_heads=0), 1, b"multiple of kv_heads"),
     (dict(kv_heads=0), 1, b"cache extents"),
     (dict(q_heads=258), 2, b"query heads per KV head"),
     (dict(batch=0), 1, b"batch"),
     (dict(total_q=-1), 1, b"batch"),
-    (dict(prefix=-1), 1, b"extents"),
-    (dict(cols=5), 1, b"extents"),
-    (dict(cols=0), 1, b"extents"),
+    (dict(prefix_len=-1), 1, b"extents"),
+    (dict(table_cols=5), 1, b"extents"),
+    (dict(table_cols=0), 1, b"extents"),
     (dict(scale=0.0), 1, b"scale"),
     (dict(scale=float("inf")), 1, b"scale"),
     (dict(scale=float("nan")), 1, b"scale"),
-    (dict(stride=2 * 16 * 128 - 8), 1, b"block_stride"),
-    (dict(stride=2 * 16 * 128 + 4), 1, b"block_stride"),
-    (dict(k=A + 8), 1, b"16-byte"),
-    (dict(v=None), 1, b"null cache"),
-    (dict(Q=None), 1, b"null"),
-    (dict(ptable=None), 1, b"null"),
-    (dict(Q=A + 2), 1, b"16-byte"),
+    (dict(block_stride=2 * 16 * 128 - 8), 1, b"block_stride"),
+    (dict(block_stride=2 * 16 * 128 + 4), 1, b"block_stride"),
+    (dict(k_cache=A + 8), 1, b"16-byte"),
+    (dict(v_cache=None), 1, b"null cache"),
+    (dict(q=None), 1, b"null"),
+    (dict(prefix_table=None), 1, b"null"),
+    (dict(q=A + 2), 1, b"16-byte"),
     (dict(ldq=1028), 1, b"16-byte"),
     (dict(ldo=512), 1, b"16-byte"),
     (dict(total_q=1 << 29), 1, b"extents"),
-    (dict(blocks=0), 1, b"cache extents"),
+    (dict(num_blocks=0), 1, b"cache extents"),
+    (dict(kv_heads=40000, q_heads=40000, ldq=40000 * 128, ldo=40000 * 128,
+          block_stride=40000 * 16 * 128), 1, b"extents"),
 ])
 def test_attention_paged_refuses(pkg, kw, status, text):
     lib = pkg._native.load()
-    assert attention(lib, **kw) == status
+    assert attention(pkg, **kw) == status
     assert text in lib.hxb_last_error_message()
 
 
 def test_attention_paged_without_tokens_is_nothing(pkg):
-    assert attention(pkg._native.load(), total_q=0, Q=None, O=None, ws=None, ws_bytes=0) == 0
+    assert attention(pkg, total_q=0, q=None, out=None, workspace=None, workspace_bytes=0) == 0
+
+
+def test_attention_paged_arguments_have_the_layout_of_the_wrapper(pkg):
+    """The Python entry packs the argument record by itself."""
+    native = pkg._native.AttentionPaged
+    assert pkg.paged._ARGUMENTS.size == ctypes.sizeof(native)
+    values = list(range(1, 23)) + [0.5, 24, 25, 26]
+    got = native.from_buffer_copy(pkg.paged._ARGUMENTS.pack(*values))
+    assert [getattr(got, f[0]) for f in native._fields_] == values
+    assert pkg._native.load().hxb_attention_paged_f16(None, None) == 1
 
 
 def tables(lib, **kw):
