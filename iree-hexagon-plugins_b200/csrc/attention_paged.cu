@@ -11,10 +11,10 @@
 // keys together, while each request's rows walk its own keys.
 //
 // Two kernels share the work (paged_work.cuh says how it is cut): the narrow one
-// (attention_paged_narrow.cuh, keys on the TMEM lanes, bound by HBM) takes
-// requests of at most 16 rows per KV head, the wide one (attention_paged_wide.cuh,
-// rows on the lanes, bound by the tensor core) the others and a prefix that many
-// rows share. A combine kernel merges what each row has. K and V blocks come
+// (attention_paged_narrow.cuh, keys on the TMEM lanes, bound by HBM) takes the
+// own keys of decode batches, at most 16 rows per KV head and request, the wide
+// one (attention_paged_wide.cuh, rows on the lanes, bound by the tensor core)
+// those of other batches and a prefix that many rows share. A combine kernel merges what each row has. K and V blocks come
 // through 3-D tensor maps, one TMA box per cache block and 64 columns, straight
 // into the 128B-swizzled tile.
 //
@@ -42,22 +42,24 @@ constexpr int kNarrowPrefixRows = 64;
 constexpr int kWideUnitCost = 2;
 
 // Merges the partials of every row: a block has 32 packed rows of one KV head
-// (lane = row) and 64 columns (warp = 8 of them), so that partials, which lie
-// row by row in groups of four columns, are read in whole lines. A row has one
-// partial per CTA that walked a part of its prefix keys or of its own keys; a row
-// without any key is 0.
-constexpr int kCombineThreads = 256;
+// (lane = row) and 32 columns (warp = 8 of them), so that partials, which lie
+// row by row in groups of four columns, are read in whole lines, eight pieces in
+// flight at a time. A row has one partial per CTA that walked a part of its
+// prefix keys or of its own keys; a row without any key is 0.
+constexpr int kCombineThreads = 128;
+constexpr int kCombineCols = kCombineThreads / 32 * 8;
 
 template <int D>
 __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kernel(const PagedArgs a) {
   pdl_wait();
   pdl_trigger();
-  constexpr int kColBlocks = D / 64;
+  constexpr int kColBlocks = D / kCombineCols;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h = blockIdx.y / kColBlocks;
-  const int v0 = blockIdx.y % kColBlocks * 16 + warp * 2;  // first of two float4 columns
-  const long long R = (long long)a.total_q * a.group;
-  const long long pr = (long long)blockIdx.x * 32 + lane;
+  // first of this warp's two float4 columns
+  const int v0 = blockIdx.y % kColBlocks * (kCombineCols / 4) + warp * 2;
+  const int R = a.total_q * a.group;
+  const int pr = blockIdx.x * 32 + lane;
   // the lengths and tables of the call, checked once
   if (blockIdx.x == 0 && blockIdx.y == 0) {
     bool bad = false;
@@ -67,85 +69,82 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
     if (bad) atomicOr(a.status, kStatusBadIndex);
   }
   if (pr >= R) return;
-  const long long at = h * R + pr;
+  const long long at = (long long)h * R + pr;
   const int2 own = a.info[0][at];
   const int2 pre = a.prefix_len > 0 ? a.info[1][at] : make_int2(0, 0);
-  const int tok = (int)(pr / a.group);
+  const int tok = pr / a.group;
   if (tok < clamp_token(a, 0) || tok >= clamp_token(a, a.batch)) return;
-  const int n_own = own.y & 0xffff, n_pre = pre.y & 0xffff;
   const bool prefix = a.prefix_len > 0 && !(own.x & kWithPrefix);
+  const int n_own = own.y & 0xffff, n_pre = prefix ? pre.y & 0xffff : 0;
   if (!prefix && n_own == 1) return;  // written by the attention kernel
+  // (records left unwritten by a launch that gave up on a wait)
+  auto wrong = [&](int2 info, int n) {
+    const bool narrow = (info.x & kNarrowSlot) != 0;
+    return n < 1 || info.x < 0 || (unsigned)info.y >> 16 >= (narrow ? 16u : 256u) ||
+           (info.x & (kWithPrefix - 1)) + n > a.ctas[narrow];
+  };
+  if (wrong(own, n_own) || (prefix && wrong(pre, n_pre))) return;
+  const int pieces = n_own + n_pre;
   float m = -INFINITY, sum = 0.0f;
   float acc[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-  bool wrong = false;
-  auto merge = [&](int set, int2 info, int n) {
-    const bool narrow = (info.x & kNarrowSlot) != 0;
-    const int first = info.x & (kWithPrefix - 1), prow = info.y >> 16;
-    const int rows = narrow ? kNarrowRows : 256;
-    // (records left unwritten by a launch that gave up on a wait)
-    if (n < 1 || info.x < 0 || (unsigned)prow >= (unsigned)rows || first + n > a.ctas[narrow]) {
-      wrong = true;
-      return;
-    }
-    const float* cut_o = narrow ? a.cut_o[1] : a.cut_o[0];
-    const float* cut_lse = narrow ? a.cut_lse[1] : a.cut_lse[0];
-    constexpr int kBatch = 4;
+  constexpr int kBatch = 8;
 #pragma unroll 1
-    for (int p0 = 0; p0 < n; p0 += kBatch) {
-      float lse[kBatch];
-      float4 x[kBatch][2];
+  for (int p0 = 0; p0 < pieces; p0 += kBatch) {
+    float lse[kBatch];
+    float4 x[kBatch][2];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int p = p0 + i;
-        lse[i] = -INFINITY;
-        if (p >= n) continue;
-        const float* src;
-        long long pitch;
+    for (int i = 0; i < kBatch; ++i) {
+      lse[i] = -INFINITY;
+      if (p0 + i < pieces) {
+        const bool set = p0 + i >= n_own;
+        const int2 info = set ? pre : own;
+        const int n = set ? n_pre : n_own, p = set ? p0 + i - n_own : p0 + i;
+        const float *src, *stat;
+        int pitch;
         if (n == 1) {
-          src = a.whole_o[set] + ((h * (D / 4) + v0) * R + pr) * 4;
-          pitch = R * 4;
-          lse[i] = a.whole_lse[set][at];
+          src = a.whole_o[set] + ((long long)h * (D / 4) * R + pr) * 4;
+          stat = a.whole_lse[set] + at;
+          pitch = R;
         } else {
-          const long long slot = p == 0 ? 2 * first + 1 : 2 * (first + p);
-          src = cut_o + (slot * D + v0 * 4) * rows + prow * 4;
-          pitch = rows * 4;
-          lse[i] = cut_lse[slot * rows + prow];
+          const bool narrow = (info.x & kNarrowSlot) != 0;
+          pitch = narrow ? kNarrowRows : 256;
+          const int cta = (info.x & (kWithPrefix - 1)) + p;
+          const int row = (2 * cta + (p == 0)) * pitch + (info.y >> 16);
+          stat = a.cut_lse[narrow] + row;
+          src = a.cut_o[narrow] + ((long long)(2 * cta + (p == 0)) * (D / 4) * pitch + (info.y >> 16)) * 4;
         }
-        x[i][0] = *reinterpret_cast<const float4*>(src);
-        x[i][1] = *reinterpret_cast<const float4*>(src + pitch);
-      }
-      float m_new = m;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, lse[i]);
-      const float scale = m == -INFINITY ? 0.0f : ex2_approx(m - m_new);
-      // (nothing visible so far, or only NaN: acc and sum are 0 or NaN)
-      if (m != -INFINITY) {
-        sum *= scale;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] *= scale;
-      }
-      m = m_new;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        if (lse[i] == -INFINITY) continue;
-        const float w = ex2_approx(lse[i] - m);
-        sum += w;
-        acc[0] = fmaf(w, x[i][0].x, acc[0]);
-        acc[1] = fmaf(w, x[i][0].y, acc[1]);
-        acc[2] = fmaf(w, x[i][0].z, acc[2]);
-        acc[3] = fmaf(w, x[i][0].w, acc[3]);
-        acc[4] = fmaf(w, x[i][1].x, acc[4]);
-        acc[5] = fmaf(w, x[i][1].y, acc[5]);
-        acc[6] = fmaf(w, x[i][1].z, acc[6]);
-        acc[7] = fmaf(w, x[i][1].w, acc[7]);
+        lse[i] = *stat;
+        x[i][0] = *reinterpret_cast<const float4*>(src + (long long)v0 * pitch * 4);
+        x[i][1] = *reinterpret_cast<const float4*>(src + (long long)(v0 + 1) * pitch * 4);
       }
     }
-  };
-  merge(0, own, n_own);
-  if (prefix) merge(1, pre, n_pre);
-  if (wrong) return;
+    float m_new = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, lse[i]);
+    if (m != -INFINITY) {  // (nothing visible so far: sum and acc are 0, or NaN)
+      const float scale = ex2_approx(m - m_new);
+      sum *= scale;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= scale;
+    }
+    m = m_new;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (lse[i] == -INFINITY) continue;
+      const float w = ex2_approx(lse[i] - m);
+      sum += w;
+      acc[0] = fmaf(w, x[i][0].x, acc[0]);
+      acc[1] = fmaf(w, x[i][0].y, acc[1]);
+      acc[2] = fmaf(w, x[i][0].z, acc[2]);
+      acc[3] = fmaf(w, x[i][0].w, acc[3]);
+      acc[4] = fmaf(w, x[i][1].x, acc[4]);
+      acc[5] = fmaf(w, x[i][1].y, acc[5]);
+      acc[6] = fmaf(w, x[i][1].z, acc[6]);
+      acc[7] = fmaf(w, x[i][1].w, acc[7]);
+    }
+  }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   uint4 o;
   o.x = pack_half2(acc[0] * inv, acc[1] * inv);
@@ -215,35 +214,35 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
                           cudaStream_t stream) {
   hxb_status_t s = configure_paged<D>(dev);
   if (s != HXB_OK) return s;
-  // Requests of at most 16 rows per KV head go to the narrow kernel; where no
-  // request is expected to have more, all of them do.
+  // Batches whose requests are expected to have at most 16 rows per KV head go to
+  // the narrow kernel, others to the wide one (its solo mode is as near to HBM
+  // on a long request; a launch of the narrow kernel for the short requests of a
+  // mixed batch cost more than it saved).
   const int narrow_tok = kNarrowRows / a.group;
-  const bool all_narrow = narrow_tok > 0 && max_q_len <= narrow_tok;
+  const bool narrow = narrow_tok > 0 && max_q_len <= narrow_tok;
   const bool prefix = a.prefix_len > 0;
   const bool narrow_prefix =
-      prefix && narrow_tok > 0 && (int64_t)a.total_q * a.group <= kNarrowPrefixRows;
-  if (!all_narrow || (prefix && !narrow_prefix)) {
+      narrow && prefix && (int64_t)a.total_q * a.group <= kNarrowPrefixRows;
+  if (!narrow || (prefix && !narrow_prefix)) {
     PagedArgs w = a;
     w.unit_tok = 2 * a.tile_tok;
-    w.min_tok = all_narrow ? 1 : narrow_tok + 1;
-    w.max_tok = all_narrow ? 0 : INT32_MAX;
-    w.prefix_here = prefix && !narrow_prefix;
-    w.fat_tok = !all_narrow && w.prefix_here ? a.tile_tok : 0;
     w.unit_cost = kWideUnitCost;
+    w.requests_here = !narrow;
+    w.prefix_here = prefix;
+    w.fat_tok = !narrow && prefix ? a.tile_tok : 0;
     s = launch_pdl(attention_paged_wide_kernel<D>, dim3((unsigned)dev.num_sms), dim3(kThreads),
                    WideSmem<D>::kAlloc, stream, "paged attention launch", tmQ, tmK, tmV, w);
     if (s != HXB_OK) return s;
   }
-  if (narrow_tok > 0) {
+  if (narrow) {
     PagedArgs n = a;
     // rows of a unit: what the largest request, and a prefix, can fill
-    int64_t rows = all_narrow ? std::max<int64_t>(1, max_q_len) * a.group : kNarrowRows;
+    int64_t rows = std::max<int64_t>(1, max_q_len) * a.group;
     if (narrow_prefix)
       rows = std::max(rows, std::min<int64_t>((int64_t)a.total_q * a.group, kNarrowRows));
     const int nr = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     n.unit_tok = nr / a.group;
-    n.min_tok = 0;
-    n.max_tok = all_narrow ? INT32_MAX : narrow_tok;
+    n.requests_here = 1;
     n.prefix_here = narrow_prefix;
     const auto kernel = nr == 4   ? attention_paged_narrow_kernel<D, 4>
                         : nr == 8 ? attention_paged_narrow_kernel<D, 8>
@@ -254,7 +253,7 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   }
   const int64_t chunks = ((int64_t)a.total_q * a.group + 31) / 32;
   return launch_pdl(attention_paged_combine_kernel<D>,
-                    dim3((unsigned)chunks, (unsigned)(a.kv_heads * (D / 64))),
+                    dim3((unsigned)chunks, (unsigned)(a.kv_heads * (D / kCombineCols))),
                     dim3(kCombineThreads), 0, stream, "paged attention combine launch", a);
 }
 
@@ -294,7 +293,7 @@ extern "C" hxb_status_t hxb_attention_paged_f16(const hxb_attention_paged_t* arg
   if (group > kBM)
     return fail(HXB_STATUS_UNSUPPORTED, "paged attention: %lld query heads per KV head (at most %d)",
                 (long long)group, kBM);
-  if (kv_heads * (head_dim / 64) > 65535 || total_q > INT32_MAX / q_heads || table_cols < 1 || table_ld < table_cols ||
+  if (kv_heads * (head_dim / kCombineCols) > 65535 || total_q > INT32_MAX / q_heads || table_cols < 1 || table_ld < table_cols ||
       table_cols > INT32_MAX / 2 / block_rows || prefix_len < 0 || prefix_len > INT32_MAX / 2)
     return fail(HXB_STATUS_INVALID_ARGUMENT, "paged attention: bad extents");
   if (!(scale > 0.0f) || !isfinite(scale))

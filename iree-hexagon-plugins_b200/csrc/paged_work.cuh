@@ -55,7 +55,7 @@ struct PagedArgs {
   int total_q, batch, q_heads, kv_heads, group;
   int unit_tok;            // tokens per row unit
   int unit_cost;           // blocks that its start and end cost
-  int min_tok, max_tok;    // this kernel takes the requests of that many tokens
+  int requests_here;       // this kernel takes the requests' own keys
   int prefix_here;         // and the prefix
   int fat_tok;             // requests of so many tokens fill tiles (0: no matter)
   int tile_tok, box_tok;   // wide kernel: tokens per 128-row tile and per Q box
@@ -175,7 +175,6 @@ __device__ __forceinline__ Segment own_segment(const PagedArgs& a, int b, int pr
   Segment s;
   s.tok = clamp_token(a, b);
   s.n = own_tokens(a, b);
-  if (s.n < a.min_tok || s.n > a.max_tok) s.n = 0;  // the other kernel's
   s.keys = (int)min((long long)max(a.kv_lens[b], 0), (long long)a.table_cols << a.rows_log2);
   s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
   s.pre = pre;
@@ -214,7 +213,7 @@ struct ShareSmem {
 template <int THREADS>
 __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREADS>& sm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = a.min_tok <= a.max_tok ? (a.batch + THREADS - 1) / THREADS : 0;
+  const int each = a.requests_here ? (a.batch + THREADS - 1) / THREADS : 0;
   const int b0 = min((int)threadIdx.x * each, a.batch), b1 = min(b0 + each, a.batch);
   // every request fills tiles by itself: no shared pass over the prefix
   bool fat = false;
