@@ -152,18 +152,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (item.blocks == 0) continue;
         const bool pair = item.ntok > args.tile_tok;
         const int la = pair ? 1 : 2;  // K blocks ahead of the V block
-        auto load_tile = [&](const CUtensorMap* map, int j) -> bool {
-          // (the block id is on its way while the slot is waited for)
-          const BlockOf at = block_at(args, item, item.j0 + j);
-          const int block = loader.block_of(args, at.keys, at.table, at.j);
-          const int slot = ring.slot();
-          if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[slot], ring.parity() ^ 1, fs)))
-            return false;
-          loader.load(args, item.head, map, smem + L::kOffKV + slot * kTileBytes, &kv_full[slot],
-                      at.j, block);
-          ++ring.n;
-          return true;
-        };
         // Q of the row unit (a second tile begins where the first one's boxes
         // end: tile_tok is a multiple of box_tok)
         if (!__all_sync(0xffffffffu, mbar_wait(q_empty, (q_items & 1) ^ 1, fs))) break;
@@ -179,10 +167,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_load_3d(smem + L::kOffQ + t * kTileBytes + half * kBoxBytes + bx * box_bytes, &tmQ,
                       q_full, 64 * half, item.head * args.group, item.tok0 + q * args.box_tok);
         }
-        for (int j = 0; j < min(la, item.blocks) && ok; ++j) ok = load_tile(&tmK, j);
-        for (int j = 0; j < item.blocks && ok; ++j) {
-          ok = load_tile(&tmV, j);
-          if (ok && j + la < item.blocks) ok = load_tile(&tmK, j + la);
+        // V block j behind K block j + la (the first la K blocks by themselves)
+#pragma unroll 1
+        for (int i = -2 * la; i < 2 * item.blocks && ok; ++i) {
+          const int which = !(i & 1);  // V_j, then K_{j + la}
+          const int j = which ? i >> 1 : (i >> 1) + la;
+          if (j < 0 || j >= item.blocks) continue;
+          const BlockOf at = block_at(args, item, item.j0 + j);
+          // (the block id is on its way while the slot is waited for)
+          const int block = loader.block_of(args, at.keys, at.table, at.j);
+          const int slot = ring.slot();
+          ok = __all_sync(0xffffffffu, mbar_wait(&kv_empty[slot], ring.parity() ^ 1, fs));
+          if (!ok) break;
+          loader.load(args, item.head, which ? &tmV : &tmK, smem + L::kOffKV + slot * kTileBytes,
+                      &kv_full[slot], at.j, block);
+          ++ring.n;
         }
       }
       // bounded wait for the copies still landing (complete on the normal path)
@@ -217,85 +216,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
           ok = mbar_wait(q_full, q_items & 1, fs);
           const bool pair = item.ntok > args.tile_tok;
-          const int nb = item.blocks;
-          auto wait_tile = [&]() -> bool {
-            const bool r = mbar_wait(&kv_full[ring.slot()], ring.parity(), fs);
-            tc_fence_after();
-            return r;
-          };
-          auto issue_s = [&](int t, int q, int slot) {
-            const uint64_t kd = k_desc + slot * kTileStep;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              umma_f16_ss(tmem_base + t * 128, q_desc + q * kTileStep + kstep(kk), kd + kstep(kk),
-                          kIdescQK, kk != 0);
-            umma_commit(&s_full[t]);
-            issued_any = true;
-          };
-          auto issue_pv = [&](int t, int slot, bool fresh) {
-            const uint64_t vd = v_desc + slot * kTileStep;
-#pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)
-              umma_f16_ts(tmem_base + 256 + t * D, tmem_base + t * 128 + 64 + kk * 8,
-                          vd + (uint64_t)(kk * 16 * 128 >> 4), kIdescPV, !fresh || kk != 0);
-          };
-          auto wait_p = [&](int t) -> bool {
-            const bool r = mbar_wait(&p_full[t], (p_par >> t) & 1, fs);
-            p_par ^= 1u << t;
-            tc_fence_after();
-            return r;
-          };
-          auto wait_fix = [&]() -> bool { return mbar_wait(v_ready, fixes++ & 1, fs); };
-          const int la = pair ? 1 : 2;
-          // S of the first block(s)
-          for (int j = 0; j < min(la, nb) && ok; ++j) {
-            if (!(ok = wait_tile())) break;
-            const int slot = ring.slot();
-            if (pair) {
-              issue_s(0, 0, slot);
-              issue_s(1, 1, slot);
-            } else {
-              issue_s(j, 0, slot);
-            }
-            umma_commit(&kv_empty[slot]);
-            ++ring.n;
-          }
-          if (ok && nb <= la) umma_commit(q_empty);
-          for (int j = 0; j < nb && ok; ++j) {
-            const int vslot = ring.slot();
-            if (!(ok = wait_tile())) break;
-            ++ring.n;
-            const int rows = block_rows_at(args, item, item.j0 + j);
-            const bool fix = rows < kBN;
-            if (fix) {  // (zeroed while the softmax runs)
-              *v_job = vslot << 8 | rows;
-              mbar_arrive(v_need);
-            }
-            // both warpgroups have read the previous item's accumulators
-            if (j == 0 && q_items && !(ok = mbar_wait(o_free, (q_items & 1) ^ 1, fs))) break;
+          const int nb = item.blocks, la = pair ? 1 : 2;
+          // Step j: PV of block j and S of block j + la, for both tiles (pair) or
+          // for stream j mod 2 (solo).
+#pragma unroll 1
+          for (int j = -la; j < nb && ok; ++j) {
             const bool more = j + la < nb;
+            const int vslot = ring.slot();
+            bool fix = false;
+            if (j >= 0) {
+              if (!(ok = mbar_wait(&kv_full[vslot], ring.parity(), fs))) break;
+              ++ring.n;
+              const int rows = block_rows_at(args, item, item.j0 + j);
+              fix = rows < kBN;
+              if (fix) {  // (zeroed while the softmax runs)
+                *v_job = vslot << 8 | rows;
+                mbar_arrive(v_need);
+              }
+              // both warpgroups have read the previous item's accumulators
+              if (j == 0 && q_items && !(ok = mbar_wait(o_free, (q_items & 1) ^ 1, fs))) break;
+            }
             const int kslot = ring.slot();
-            if (pair) {
-              if (more && !(ok = wait_tile())) break;
-              if (!(ok = wait_p(0))) break;
-              if (fix && !(ok = wait_fix())) break;
-              issue_pv(0, vslot, j == 0);
-              if (more) issue_s(0, 0, kslot);
-              if (!(ok = wait_p(1))) break;
-              issue_pv(1, vslot, j == 0);
-              umma_commit(&kv_empty[vslot]);
-              if (more) issue_s(1, 1, kslot);
-            } else {
-              const int t = j & 1;
-              if (!(ok = wait_p(t))) break;
-              if (fix && !(ok = wait_fix())) break;
-              issue_pv(t, vslot, j < 2);
-              umma_commit(&kv_empty[vslot]);
+            bool k_here = false;
+            const int t0 = pair ? 0 : j & 1, t1 = pair ? 1 : t0;
+#pragma unroll 1
+            for (int t = t0; t <= t1; ++t) {
+              if (j >= 0) {
+                if (!(ok = mbar_wait(&p_full[t], (p_par >> t) & 1, fs))) break;
+                p_par ^= 1u << t;
+                if (fix && t == t0 && !(ok = mbar_wait(v_ready, fixes++ & 1, fs))) break;
+                tc_fence_after();
+                const uint64_t vd = v_desc + vslot * kTileStep;
+#pragma unroll
+                for (int kk = 0; kk < kBN / 16; ++kk)
+                  umma_f16_ts(tmem_base + 256 + t * D, tmem_base + t * 128 + 64 + kk * 8,
+                              vd + (uint64_t)(kk * 16 * 128 >> 4), kIdescPV, j >= la || kk != 0);
+                if (t == t1) umma_commit(&kv_empty[vslot]);
+              }
               if (more) {
-                if (!(ok = wait_tile())) break;
-                issue_s(t, 0, kslot);
+                if (!k_here && !(ok = mbar_wait(&kv_full[kslot], ring.parity(), fs))) break;
+                k_here = true;
+                tc_fence_after();
+                const uint64_t qd = q_desc + (pair ? t : 0) * kTileStep;
+                const uint64_t kd = k_desc + kslot * kTileStep;
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk)
+                  umma_f16_ss(tmem_base + t * 128, qd + kstep(kk), kd + kstep(kk), kIdescQK,
+                              kk != 0);
+                umma_commit(&s_full[t]);
+                issued_any = true;
               }
             }
+            if (!ok) break;
             if (more) {
               umma_commit(&kv_empty[kslot]);
               ++ring.n;
@@ -359,30 +331,42 @@ __global__ void __launch_bounds__(kThreads, 1)
       return __all_sync(0xffffffffu, ok);
     };
     bool ok = true;
+    // The first pass has no item: it runs the block's instructions once on
+    // whatever the O columns hold (the first PV rewrites them), while the first
+    // loads are under way, so that the first block does not wait for 12 KB of
+    // instruction fetches.
+    bool warm = true;
     // The item stays in shared memory while it is worked on (its registers
     // hold a row of scores) and is released at its end.
+#pragma unroll 1
     while (ok) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&item_full[it.slot()], it.parity(), fs))) break;
       const volatile Item& item = items[it.slot()];
-      if (item.request == kEnd) break;
-      const bool pair = item.ntok > args.tile_tok;
+      if (!warm) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&item_full[it.slot()], it.parity(), fs))) break;
+        if (item.request == kEnd) break;
+      }
+      const bool pair = warm || item.ntok > args.tile_tok;
       // the row's token within the unit, and whether the tile has that row
       auto token = [&]() { return (pair ? t * args.tile_tok : 0) + r / args.group; };
       auto is_live = [&]() { return r < args.tile_tok * args.group && token() < item.ntok; };
-      const bool warp_live = __any_sync(0xffffffffu, is_live());
+      const bool warp_live = warm || __any_sync(0xffffffffu, is_live());
+      const int nb = warm ? t + 1 : item.blocks;
       float m_run = -INFINITY;  // running max of S*c (log2 domain)
       float l_run = 0.0f;       // running sum of P against m_run
-      for (int j = pair ? 0 : t; j < item.blocks; j += pair ? 1 : 2) {
-        const bool ready = mbar_wait(&s_full[t], ph & kS, fs);
-        ph ^= kS;
-        if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
-        tc_fence_after();
+#pragma unroll 1
+      for (int j = pair && !warm ? 0 : t; j < nb; j += pair ? 1 : 2) {
+        if (!warm) {
+          const bool ready = mbar_wait(&s_full[t], ph & kS, fs);
+          ph ^= kS;
+          if (!__all_sync(0xffffffffu, ready)) { ok = false; break; }
+          tc_fence_after();
+        }
         if (warp_live) {
           float s[kBN];
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) {
             uint32_t u[32];
-            tmem_ld_32x32b_x32(lane_base + s_col + ch * 32, u);
+            tmem_ld_32x32b_x32(lane_base + (warm ? o_col : s_col) + ch * 32, u);
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[ch * 32 + e] = __uint_as_float(u[e]);
           }
@@ -448,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               acc2[e & 1] = f2_add(acc2[e & 1], f2_pack(p0, p1));
               pk[e] = pack_half2(p0, p1);
             }
-            tmem_st_32x32b_x32(lane_base + p_col + h * 32, pk);
+            tmem_st_32x32b_x32(lane_base + (warm ? o_col : p_col) + h * 32, pk);
           }
           float sa, sb, sc2, sd;
           f2_unpack(acc2[0], sa, sb);
@@ -456,10 +440,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           l_run += (sa + sb) + (sc2 + sd);
           tmem_wait_st();
         }
+        if (warm) break;
         tc_fence_before();
         mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
+      if (warm) {
+        warm = false;
+        continue;
+      }
       // -------------------------------------------------------- epilogue
       const int blocks = item.blocks;
       const int tok = token();
@@ -522,38 +511,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                      (long long)(item.head * args.group + r % args.group) * D;
       if (warp_live) {
 #pragma unroll 1
-        for (int ch = 0; ch < cols / 32; ++ch) {
-          uint32_t u[32];
+        for (int ch = 0; ch < cols; ch += 16) {
+          uint32_t u[16];
+          float o[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+          // (an accumulator whose row sum is 0 is 0: its weight may be 0)
           if (blocks > 0) {
-            tmem_ld_32x32b_x32(lane_base + a0_col + col0 + ch * 32, u);
+            tmem_ld_32x32b_x16(lane_base + a0_col + col0 + ch, u);
             tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(u[e]) * w0;
           }
-          float o[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = w0 == 0.0f ? 0.0f : __uint_as_float(u[e]) * w0;
           if (!pair && blocks > 1) {
-            tmem_ld_32x32b_x32(lane_base + 256 + D + col0 + ch * 32, u);
+            tmem_ld_32x32b_x16(lane_base + 256 + D + col0 + ch, u);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              o[e] = w1 == 0.0f ? o[e] : fmaf(__uint_as_float(u[e]), w1, o[e]);
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(__uint_as_float(u[e]), w1, o[e]);
           }
           if (!live) continue;
           if (direct) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int v = 0; v < 2; ++v) {
               uint4 x;
               x.x = pack_half2(o[v * 8 + 0], o[v * 8 + 1]);
               x.y = pack_half2(o[v * 8 + 2], o[v * 8 + 3]);
               x.z = pack_half2(o[v * 8 + 4], o[v * 8 + 5]);
               x.w = pack_half2(o[v * 8 + 6], o[v * 8 + 7]);
-              *reinterpret_cast<uint4*>(orow + col0 + ch * 32 + v * 8) = x;
+              *reinterpret_cast<uint4*>(orow + col0 + ch + v * 8) = x;
             }
           } else {
+            float* to = dst + (long long)((col0 + ch) / 4) * pitch;
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<float4*>(dst + (long long)((col0 + ch * 32) / 4 + v) * pitch) =
+            for (int v = 0; v < 4; ++v) {
+              *reinterpret_cast<float4*>(to) =
                   make_float4(o[v * 4], o[v * 4 + 1], o[v * 4 + 2], o[v * 4 + 3]);
+              to += pitch;
+            }
           }
         }
       }

@@ -132,39 +132,42 @@ __device__ __forceinline__ int unit_blocks(const PagedArgs& a, const Segment& s,
 // sum_{i < n} floor((a i + b) / m), by the Euclidean algorithm on (a, m): whole
 // multiples of m leave the sum in closed form, and what is left counts the
 // lattice points under a line, which swapping the axes turns into a shorter sum.
-__device__ __forceinline__ long long floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
-  long long sum = 0;
+// The caller bounds the result (and so every term) below 2^31.
+__device__ __forceinline__ unsigned floor_sum(unsigned n, unsigned m, unsigned a, unsigned b) {
+  unsigned sum = 0;
+#pragma unroll 1
   while (true) {
-    sum += (long long)n * (n - 1) / 2 * (a / m) + (long long)n * (b / m);
-    a %= m;
-    b %= m;
+    const unsigned qa = a / m, qb = b / m;
+    // (one of n, n - 1 is even; qa is 0 after the first round or n is short)
+    sum += (n & 1 ? (n - 1) / 2 * n : n / 2 * (n - 1)) * qa + n * qb;
+    a -= qa * m;
+    b -= qb * m;
     const unsigned top = a * n + b;  // (a, b < m <= 256: below 2^32)
     if (top < m) return sum;
     n = top / m;
-    b = top % m;
+    b = top - n * m;
     const unsigned t = m;
     m = a;
     a = t;
   }
 }
 
-constexpr int kMostWork = 1 << 30;  // blocks of one call (saturated above)
+constexpr int kMostWork = 1 << 30;  // units of work of one call (saturated above)
 
 // Work of the first `units` row units of one KV head.
 __device__ __forceinline__ int work_before(const PagedArgs& a, const Segment& s, int units) {
-  long long sum = (long long)units * a.unit_cost;
-  if (units <= 1 || !s.causal) {
-    if (units) sum += (long long)units * unit_blocks(a, s, 0);
-  } else {
-    // unit u < units - 1 sees d + (u + 1) T own keys: none up to u = dark, then
-    // one block per begun 128
-    const int T = a.unit_tok, d = s.keys - s.n, full = units - 1;
-    const int dark = d < 0 ? min(full, (-d) / T) : 0;
-    sum += (long long)dark * max(1, s.pre) + (long long)(full - dark) * s.pre;
-    if (full > dark) sum += floor_sum(full - dark, kBN, T, d + (dark + 1) * T + kBN - 1);
-    sum += unit_blocks(a, s, full);
-  }
-  return (int)min(sum, (long long)kMostWork);
+  if (units == 0) return 0;
+  const int last = unit_blocks(a, s, units - 1);  // the most blocks of a unit
+  if ((float)units * (float)(last + a.unit_cost) >= (float)kMostWork) return kMostWork;
+  int sum = units * a.unit_cost + last;
+  if (!s.causal) return sum + (units - 1) * last;
+  // unit u < units - 1 sees d + (u + 1) T own keys: none up to u = dark, then one
+  // block per begun 128
+  const int T = a.unit_tok, d = s.keys - s.n, full = units - 1;
+  const int dark = d < 0 ? min(full, (-d) / T) : 0;
+  sum += dark * max(1, s.pre) + (full - dark) * s.pre;
+  if (full > dark) sum += (int)floor_sum(full - dark, kBN, T, d + (dark + 1) * T + kBN - 1);
+  return sum;
 }
 
 __device__ __forceinline__ int own_tokens(const PagedArgs& a, int b) {
@@ -228,56 +231,59 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
   }
   Share r{0, 0, 1, fat ? (a.prefix_len + kBN - 1) / kBN : 0};
   const Segment pre = prefix_segment(a, a.prefix_here && !fat);
-  long long mine = 0;
-  Segment s;
+  const int pre_work = (int)min((long long)pre.work * a.kv_heads, (long long)kMostWork);
+  long long mine = 0, base = 0, total = pre_work;
+  // Two passes over the requests: their work, then (the thread that holds it) the
+  // CTA's first unit.
 #pragma unroll 1
-  for (int b = b0; b < b1; ++b) {
-    s = own_segment(a, b, r.pre);
-    mine += (long long)s.work * a.kv_heads;
-  }
-  long long scan = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += v;
-  }
-  if (lane == 31) sm.sum[warp] = scan;
-  __syncthreads();
-  const long long pre_work = (long long)pre.work * a.kv_heads;
-  long long total = pre_work, base = pre_work;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w == warp) base = total;
-    total += sm.sum[w];
-  }
-  base += scan - mine;
-  if (total >= kMostWork) {  // (hours of work: not started)
-    if (threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
-    return r;
-  }
-  r.per = max(1, ((int)total + (int)gridDim.x - 1) / (int)gridDim.x);
-  r.lo = min((int)blockIdx.x * r.per, (int)total);
-  r.hi = min(r.lo + r.per, (int)total);
-  if (r.lo < r.hi) {
-    if (r.lo >= base && r.lo < base + mine) {
-      int at = (int)base;
+  for (int pass = 0; pass < 2; ++pass) {
+    long long at = base;
 #pragma unroll 1
-      for (int b = b0; b < b1; ++b) {
-        if (each > 1) s = own_segment(a, b, r.pre);
-        const int w = s.work * a.kv_heads;
-        if (r.lo < at + w) {
-          sm.b = b;
-          sm.off = r.lo - at;
-          sm.seg = s;
-          break;
-        }
-        at += w;
+    for (int b = b0; b < b1; ++b) {
+      const Segment s = own_segment(a, b, r.pre);
+      const long long w = (long long)s.work * a.kv_heads;
+      at += w;
+      if (pass && r.lo < at) {
+        sm.b = b;
+        sm.off = r.lo - (int)(at - w);
+        sm.seg = s;
+        break;
       }
-    } else if (threadIdx.x == 0 && r.lo < pre_work) {
-      sm.b = -1;
-      sm.off = r.lo;
-      sm.seg = pre;
     }
+    if (pass) break;
+    mine = at;
+    if (a.requests_here) {
+      long long scan = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += v;
+      }
+      if (lane == 31) sm.sum[warp] = scan;
+      __syncthreads();
+      base = total + scan - mine;
+#pragma unroll 1
+      for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) base += sm.sum[w];
+        total += sm.sum[w];
+      }
+    }
+    if (total >= kMostWork) {  // (hours of work: not started)
+      if (threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
+      break;
+    }
+    r.per = max(1, ((int)total + (int)gridDim.x - 1) / (int)gridDim.x);
+    r.lo = min((int)blockIdx.x * r.per, (int)total);
+    r.hi = min(r.lo + r.per, (int)total);
+    if (r.lo < pre_work) {
+      if (threadIdx.x == 0) {
+        sm.b = -1;
+        sm.off = r.lo;
+        sm.seg = pre;
+      }
+      break;
+    }
+    if (r.lo >= r.hi || r.lo < base || r.lo >= base + mine) break;
   }
   __syncthreads();
   return r;
@@ -319,13 +325,14 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
     if (s.work > 0) {
       h = min(at / s.work, a.kv_heads);
       at = min(at - h * s.work, s.work - 1);
-      int above = s.units;  // work_before(u) <= at < work_before(above)
+      int above = s.units, before = 0;  // before = work_before(u) <= at < work_before(above)
+#pragma unroll 1
       while (above - u > 1) {
-        const int mid = (u + above) >> 1;
-        if (work_before(a, s, mid) <= at) u = mid;
+        const int mid = (u + above) >> 1, w = work_before(a, s, mid);
+        if (w <= at) u = mid, before = w;
         else above = mid;
       }
-      if (u) at -= work_before(a, s, u);
+      at -= before;
     }
   }
   const int cost = a.unit_cost;
