@@ -42,10 +42,11 @@ constexpr int kNarrowPrefixRows = 64;
 constexpr int kWideUnitCost = 2;
 
 // Merges the partials of every row: a block has 32 packed rows of one KV head
-// (lane = row) and 32 columns (warp = 8 of them), so that partials, which lie
-// row by row in groups of four columns, are read in whole lines, eight pieces in
-// flight at a time. A row has one partial per CTA that walked a part of its
-// prefix keys or of its own keys; a row without any key is 0.
+// (lane = row) and 32 columns (warp = 8 of them) or, where there are rows enough
+// to fill the SMs, all columns in turn; so partials, which lie row by row in
+// groups of four columns, are read in whole lines, eight pieces in flight at a
+// time. A row has one partial per CTA that walked a part of its prefix keys or of
+// its own keys; a row without any key is 0.
 constexpr int kCombineThreads = 128;
 constexpr int kCombineCols = kCombineThreads / 32 * 8;
 
@@ -53,11 +54,9 @@ template <int D>
 __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kernel(const PagedArgs a) {
   pdl_wait();
   pdl_trigger();
-  constexpr int kColBlocks = D / kCombineCols;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int h = blockIdx.y / kColBlocks;
-  // first of this warp's two float4 columns
-  const int v0 = blockIdx.y % kColBlocks * (kCombineCols / 4) + warp * 2;
+  const int col_blocks = gridDim.y / a.kv_heads;  // 1 or D / kCombineCols
+  const int h = blockIdx.y / col_blocks;
   const int R = a.total_q * a.group;
   const int pr = blockIdx.x * 32 + lane;
   // the lengths and tables of the call, checked once
@@ -85,74 +84,79 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
   };
   if (wrong(own, n_own) || (prefix && wrong(pre, n_pre))) return;
   const int pieces = n_own + n_pre;
-  float m = -INFINITY, sum = 0.0f;
-  float acc[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-  constexpr int kBatch = 8;
+  // v0: first of this warp's two float4 columns
 #pragma unroll 1
-  for (int p0 = 0; p0 < pieces; p0 += kBatch) {
-    float lse[kBatch];
-    float4 x[kBatch][2];
+  for (int v0 = blockIdx.y % col_blocks * (kCombineCols / 4) + warp * 2; v0 < D / 4;
+       v0 += col_blocks == 1 ? kCombineCols / 4 : D) {
+    float m = -INFINITY, sum = 0.0f;
+    float acc[8];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      lse[i] = -INFINITY;
-      if (p0 + i < pieces) {
-        const bool set = p0 + i >= n_own;
-        const int2 info = set ? pre : own;
-        const int n = set ? n_pre : n_own, p = set ? p0 + i - n_own : p0 + i;
-        const float *src, *stat;
-        int pitch;
-        if (n == 1) {
-          src = a.whole_o[set] + ((long long)h * (D / 4) * R + pr) * 4;
-          stat = a.whole_lse[set] + at;
-          pitch = R;
-        } else {
-          const bool narrow = (info.x & kNarrowSlot) != 0;
-          pitch = narrow ? kNarrowRows : 256;
-          const int cta = (info.x & (kWithPrefix - 1)) + p;
-          const int row = (2 * cta + (p == 0)) * pitch + (info.y >> 16);
-          stat = a.cut_lse[narrow] + row;
-          src = a.cut_o[narrow] + ((long long)(2 * cta + (p == 0)) * (D / 4) * pitch + (info.y >> 16)) * 4;
+    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
+    constexpr int kBatch = 8;
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += kBatch) {
+      float lse[kBatch];
+      float4 x[kBatch][2];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        lse[i] = -INFINITY;
+        if (p0 + i < pieces) {
+          const bool set = p0 + i >= n_own;
+          const int2 info = set ? pre : own;
+          const int n = set ? n_pre : n_own, p = set ? p0 + i - n_own : p0 + i;
+          const float *src, *stat;
+          int pitch;
+          if (n == 1) {
+            src = a.whole_o[set] + ((long long)h * (D / 4) * R + pr) * 4;
+            stat = a.whole_lse[set] + at;
+            pitch = R;
+          } else {
+            const bool narrow = (info.x & kNarrowSlot) != 0;
+            pitch = narrow ? kNarrowRows : 256;
+            const int cta = (info.x & (kWithPrefix - 1)) + p;
+            const int row = (2 * cta + (p == 0)) * pitch + (info.y >> 16);
+            stat = a.cut_lse[narrow] + row;
+            src = a.cut_o[narrow] + ((long long)(2 * cta + (p == 0)) * (D / 4) * pitch + (info.y >> 16)) * 4;
+          }
+          lse[i] = *stat;
+          x[i][0] = *reinterpret_cast<const float4*>(src + (long long)v0 * pitch * 4);
+          x[i][1] = *reinterpret_cast<const float4*>(src + (long long)(v0 + 1) * pitch * 4);
         }
-        lse[i] = *stat;
-        x[i][0] = *reinterpret_cast<const float4*>(src + (long long)v0 * pitch * 4);
-        x[i][1] = *reinterpret_cast<const float4*>(src + (long long)(v0 + 1) * pitch * 4);
+      }
+      float m_new = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, lse[i]);
+      if (m != -INFINITY) {  // (nothing visible so far: sum and acc are 0, or NaN)
+        const float scale = ex2_approx(m - m_new);
+        sum *= scale;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= scale;
+      }
+      m = m_new;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (lse[i] == -INFINITY) continue;
+        const float w = ex2_approx(lse[i] - m);
+        sum += w;
+        acc[0] = fmaf(w, x[i][0].x, acc[0]);
+        acc[1] = fmaf(w, x[i][0].y, acc[1]);
+        acc[2] = fmaf(w, x[i][0].z, acc[2]);
+        acc[3] = fmaf(w, x[i][0].w, acc[3]);
+        acc[4] = fmaf(w, x[i][1].x, acc[4]);
+        acc[5] = fmaf(w, x[i][1].y, acc[5]);
+        acc[6] = fmaf(w, x[i][1].z, acc[6]);
+        acc[7] = fmaf(w, x[i][1].w, acc[7]);
       }
     }
-    float m_new = m;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) m_new = fmaxf(m_new, lse[i]);
-    if (m != -INFINITY) {  // (nothing visible so far: sum and acc are 0, or NaN)
-      const float scale = ex2_approx(m - m_new);
-      sum *= scale;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= scale;
-    }
-    m = m_new;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (lse[i] == -INFINITY) continue;
-      const float w = ex2_approx(lse[i] - m);
-      sum += w;
-      acc[0] = fmaf(w, x[i][0].x, acc[0]);
-      acc[1] = fmaf(w, x[i][0].y, acc[1]);
-      acc[2] = fmaf(w, x[i][0].z, acc[2]);
-      acc[3] = fmaf(w, x[i][0].w, acc[3]);
-      acc[4] = fmaf(w, x[i][1].x, acc[4]);
-      acc[5] = fmaf(w, x[i][1].y, acc[5]);
-      acc[6] = fmaf(w, x[i][1].z, acc[6]);
-      acc[7] = fmaf(w, x[i][1].w, acc[7]);
-    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint4 o;
+    o.x = pack_half2(acc[0] * inv, acc[1] * inv);
+    o.y = pack_half2(acc[2] * inv, acc[3] * inv);
+    o.z = pack_half2(acc[4] * inv, acc[5] * inv);
+    o.w = pack_half2(acc[6] * inv, acc[7] * inv);
+    *reinterpret_cast<uint4*>(a.O + tok * a.ldo +
+                              ((long long)h * a.group + pr - (long long)tok * a.group) * D + v0 * 4) = o;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint4 o;
-  o.x = pack_half2(acc[0] * inv, acc[1] * inv);
-  o.y = pack_half2(acc[2] * inv, acc[3] * inv);
-  o.z = pack_half2(acc[4] * inv, acc[5] * inv);
-  o.w = pack_half2(acc[6] * inv, acc[7] * inv);
-  *reinterpret_cast<uint4*>(a.O + tok * a.ldo +
-                            ((long long)h * a.group + pr - (long long)tok * a.group) * D + v0 * 4) = o;
 }
 
 // Workspace: what the partials of a call take, in this order.
@@ -252,8 +256,9 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     if (s != HXB_OK) return s;
   }
   const int64_t chunks = ((int64_t)a.total_q * a.group + 31) / 32;
+  const int col_blocks = chunks * a.kv_heads >= 4 * dev.num_sms ? 1 : D / kCombineCols;
   return launch_pdl(attention_paged_combine_kernel<D>,
-                    dim3((unsigned)chunks, (unsigned)(a.kv_heads * (D / kCombineCols))),
+                    dim3((unsigned)chunks, (unsigned)(a.kv_heads * col_blocks)),
                     dim3(kCombineThreads), 0, stream, "paged attention combine launch", a);
 }
 

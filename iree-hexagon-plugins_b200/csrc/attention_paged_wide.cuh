@@ -19,6 +19,7 @@ namespace hxb {
 
 constexpr int kThreads = 384;
 constexpr int kItems = 4;  // items announced ahead of the roles
+constexpr int kStagePitch = 80;  // 64 bytes of a row, and 16 against bank conflicts
 // Register split of the 384 launch threads, as in attention.cu.
 constexpr int kPagedRegsLaunch = 168;
 constexpr int kPagedRegsControl = 104;
@@ -36,7 +37,8 @@ struct WideSmem {
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = kOffQ + 2 * kTileBytes;
   static constexpr int kOffML = kOffKV + kSlots * kTileBytes;  // [2][2][128] float2
-  static constexpr int kOffItems = kOffML + 4 * 128 * 8;
+  static constexpr int kOffStage = kOffML + 4 * 128 * 8;  // [8 warps][32 rows]
+  static constexpr int kOffItems = kOffStage + 8 * 32 * kStagePitch;
   static constexpr int kOffBar = kOffItems + kItems * 64;
   // q_full, q_empty, kv_full[], kv_empty[], s_full[2], p_full[2], o_full,
   // o_free, v_need, v_ready, xsync, item_full[], item_empty[], drain
@@ -507,8 +509,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                                             item.pieces | (prow << 16));
         }
       }
-      __half* orow = args.O + ((long long)item.tok0 + tok) * args.ldo +
-                     (long long)(item.head * args.group + r % args.group) * D;
+      const __half* orow = args.O + ((long long)item.tok0 + tok) * args.ldo +
+                           (long long)(item.head * args.group + r % args.group) * D + col0;
+      // Finished rows go out through shared memory, so that a store writes 64
+      // bytes of each of eight rows (a row per lane, 16 bytes at a time, took
+      // 4 us for 256 rows of 128). Lane l then has chunk l % 4 of rows l / 4 + 8 q.
+      uint8_t* stage = smem + L::kOffStage + (warp - 4) * 32 * kStagePitch;
+      const unsigned live_rows = __ballot_sync(0xffffffffu, live);
       if (warp_live) {
 #pragma unroll 1
         for (int ch = 0; ch < cols; ch += 16) {
@@ -529,7 +536,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = fmaf(__uint_as_float(u[e]), w1, o[e]);
           }
-          if (!live) continue;
           if (direct) {
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
@@ -538,9 +544,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               x.y = pack_half2(o[v * 8 + 2], o[v * 8 + 3]);
               x.z = pack_half2(o[v * 8 + 4], o[v * 8 + 5]);
               x.w = pack_half2(o[v * 8 + 6], o[v * 8 + 7]);
-              *reinterpret_cast<uint4*>(orow + col0 + ch + v * 8) = x;
+              *reinterpret_cast<uint4*>(stage + lane * kStagePitch + (ch & 16) * 2 + v * 16) = x;
             }
-          } else {
+            if (ch & 16) {
+              __syncwarp();
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int from = q * 8 + (lane >> 2);
+                __half* to = reinterpret_cast<__half*>(__shfl_sync(
+                    0xffffffffu, reinterpret_cast<unsigned long long>(orow), from));
+                const uint4 x =
+                    *reinterpret_cast<const uint4*>(stage + from * kStagePitch + (lane & 3) * 16);
+                if (live_rows >> from & 1)
+                  *reinterpret_cast<uint4*>(to + ch - 16 + (lane & 3) * 8) = x;
+              }
+              __syncwarp();
+            }
+          } else if (live) {
             float* to = dst + (long long)((col0 + ch) / 4) * pitch;
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
