@@ -102,6 +102,33 @@ __device__ __forceinline__ void tmem_st_rows(uint32_t taddr, const uint32_t (&r)
   }
 }
 
+// The largest of the warp's values (a NaN is passed over).
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Sums over the warp of N values per lane: lane l returns the sum of value
+// l / (32 / N). Half of the values change sides at each of the first steps, so
+// that N values take N - 1 + 5 - log2(N) shuffles instead of 5 N.
+template <int N>
+__device__ __forceinline__ float warp_sums(float (&v)[N], int lane) {
+  int o = 16;
+#pragma unroll
+  for (int n = N / 2; n > 0; n /= 2, o /= 2) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int q = 0; q < n; ++q) {
+      const float keep = up ? v[q + n] : v[q], give = up ? v[q] : v[q + n];
+      v[q] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+#pragma unroll
+  for (; o > 0; o /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  return v[0];
+}
+
 // NR: rows that the instance works on (4, 8 or 16; the row unit has at most that
 // many). The instruction footprint grows with it, and short requests fetch every
 // instruction for few blocks.
@@ -433,12 +460,7 @@ __global__ void __launch_bounds__(kNarThreads, 2)
           float* rd = red + (blocks_done & 1) * 64;
           float mx[NR];
 #pragma unroll
-          for (int q = 0; q < NR; ++q) mx[q] = x[q];
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-            for (int q = 0; q < NR; ++q)
-              mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], o));
+          for (int q = 0; q < NR; ++q) mx[q] = warp_max(x[q]);
           if (lane == 0)
 #pragma unroll
             for (int q = 0; q < NR; ++q) rd[quarter * 16 + q] = mx[q];
@@ -480,8 +502,10 @@ __global__ void __launch_bounds__(kNarThreads, 2)
           // zeros behind the last V row, once the tile has landed
           wait(v_need, fixes++ & 1);
           if (!bad) {
+            // (behind the end of its cache block a tile is zeros already)
+            const int P = 1 << args.rows_log2, end = min(kBN, (live + P - 1) & -P);
             uint8_t* tile = smem + L::kOffKV + *v_slot * kTileBytes;
-            for (int i = live * 8 + kl; i < kBN * 8; i += 128)
+            for (int i = live * 8 + kl; i < end * 8; i += 128)
 #pragma unroll
               for (int b = 0; b < L::kBoxes; ++b)
                 *reinterpret_cast<uint4*>(tile + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);
@@ -494,13 +518,8 @@ __global__ void __launch_bounds__(kNarThreads, 2)
       if (stop) break;
       // ---------------------------------------------------------- epilogue
       float* rl = red + 128;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int q = 0; q < NR; ++q) l_part[q] += __shfl_xor_sync(0xffffffffu, l_part[q], o);
-      if (lane == 0)
-#pragma unroll
-        for (int q = 0; q < NR; ++q) rl[quarter * 16 + q] = l_part[q];
+      const float l_sum = warp_sums<NR>(l_part, lane);
+      if (lane % (32 / NR) == 0) rl[quarter * 16 + lane / (32 / NR)] = l_sum;
       uint32_t o[NR];
       if (blocks > 0) {
         wait(o_full, items_done++ & 1);

@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int job = *v_job;
         if (job < 0) break;
         uint8_t* tile = smem + L::kOffKV + (job >> 8) * kTileBytes;
-        for (int i = (job & 255) * 8 + lane; i < kBN * 8; i += 32)
+        // (behind the end of its cache block a tile is zeros already)
+        const int P = 1 << args.rows_log2, live = job & 255, end = min(kBN, (live + P - 1) & -P);
+        for (int i = live * 8 + lane; i < end * 8; i += 32)
 #pragma unroll
           for (int b = 0; b < L::kBoxes; ++b)
             *reinterpret_cast<uint4*>(tile + b * kBoxBytes + i * 16) = make_uint4(0, 0, 0, 0);

@@ -151,6 +151,12 @@ class Batch:
     ([1] * 17, [40 * i for i in range(17)], 8, 1, 128, 16, 0, True),      # no prefix, ragged
     ([1] * 600, [(i * 7) % 40 for i in range(600)], 4, 2, 64, 16, 70, True),  # many requests
     ([1] * 2, [3000, 17], 32, 8, 128, 16, 4000, True),     # cut across many CTAs
+    # a prefix that many rows share beside short requests: both roles in one launch
+    ([1] * 9, [40 * i for i in range(9)], 16, 1, 128, 16, 300, True),
+    ([2] * 40, [2 + (i * 13) % 500 for i in range(40)], 8, 2, 128, 32, 700, True),
+    ([1] * 24, [(i * 91) % 1000 for i in range(24)], 32, 8, 64, 16, 129, True),
+    ([1] * 20, [0] * 20, 32, 8, 128, 16, 1000, True),
+    ([1, 0, 2] * 30, [(i * 7) % 300 for i in range(90)], 12, 4, 64, 16, 90, True),
     # every request fills tiles by itself: each visits the prefix before its own keys
     ([200, 150], [200, 300], 8, 2, 128, 16, 300, True),
     ([64, 100, 0, 33], [64, 10, 9, 700], 32, 8, 128, 128, 129, True),
