@@ -36,26 +36,26 @@ namespace {
 // kernel, which reads it once per 16 rows (from L2 after the first).
 constexpr int kNarrowPrefixRows = 64;
 
-// What a row unit of the wide kernel costs on top of its key blocks (Q, the first
-// softmax without an overlapping product, the epilogue), in blocks. The narrow
-// kernel hides it behind the loads of its other CTA.
+// What a row unit costs on top of its key blocks (Q, the first softmax without an
+// overlapping product, the epilogue), in blocks.
 constexpr int kWideUnitCost = 2;
+constexpr int kNarrowUnitCost = 1;
 
 // Merges the partials of every row: a block has 32 packed rows of one KV head
-// (lane = row) and 32 columns (warp = 8 of them) or, where there are rows enough
-// to fill the SMs, all columns in turn; so partials, which lie row by row in
-// groups of four columns, are read in whole lines, eight pieces in flight at a
+// (lane = row) and a group of V float4 columns per warp or, where there are rows
+// enough to fill the SMs, all columns in turn; so partials, which lie row by row
+// in groups of four columns, are read in whole lines, many pieces in flight at a
 // time. A row has one partial per CTA that walked a part of its prefix keys or of
 // its own keys; a row without any key is 0.
 constexpr int kCombineThreads = 128;
-constexpr int kCombineCols = kCombineThreads / 32 * 8;
 
-template <int D>
+template <int D, int V>
 __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kernel(const PagedArgs a) {
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col_blocks = gridDim.y / a.kv_heads;  // 1 or D / kCombineCols
+  constexpr int kStep = kCombineThreads / 32 * V;  // float4 columns of a block
+  const int col_blocks = gridDim.y / a.kv_heads;   // 1 or D / 4 / kStep
   const int h = blockIdx.y / col_blocks;
   const int R = a.total_q * a.group;
   const int pr = blockIdx.x * 32 + lane;
@@ -84,19 +84,19 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
   };
   if (wrong(own, n_own) || (prefix && wrong(pre, n_pre))) return;
   const int pieces = n_own + n_pre;
-  // v0: first of this warp's two float4 columns
+  // v0: this warp's first float4 column
 #pragma unroll 1
-  for (int v0 = blockIdx.y % col_blocks * (kCombineCols / 4) + warp * 2; v0 < D / 4;
-       v0 += col_blocks == 1 ? kCombineCols / 4 : D) {
+  for (int v0 = blockIdx.y % col_blocks * kStep + warp * V; v0 < D / 4;
+       v0 += col_blocks == 1 ? kStep : D) {
     float m = -INFINITY, sum = 0.0f;
-    float acc[8];
+    float acc[4 * V];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = 0.0f;
-    constexpr int kBatch = 8;
+    for (int e = 0; e < 4 * V; ++e) acc[e] = 0.0f;
+    constexpr int kBatch = V == 1 ? 12 : 8;
 #pragma unroll 1
     for (int p0 = 0; p0 < pieces; p0 += kBatch) {
       float lse[kBatch];
-      float4 x[kBatch][2];
+      float4 x[kBatch][V];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         lse[i] = -INFINITY;
@@ -119,8 +119,9 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
             src = a.cut_o[narrow] + ((long long)(2 * cta + (p == 0)) * (D / 4) * pitch + (info.y >> 16)) * 4;
           }
           lse[i] = *stat;
-          x[i][0] = *reinterpret_cast<const float4*>(src + (long long)v0 * pitch * 4);
-          x[i][1] = *reinterpret_cast<const float4*>(src + (long long)(v0 + 1) * pitch * 4);
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            x[i][v] = *reinterpret_cast<const float4*>(src + (long long)(v0 + v) * pitch * 4);
         }
       }
       float m_new = m;
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
         const float scale = ex2_approx(m - m_new);
         sum *= scale;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] *= scale;
+        for (int e = 0; e < 4 * V; ++e) acc[e] *= scale;
       }
       m = m_new;
 #pragma unroll
@@ -138,24 +139,23 @@ __global__ void __launch_bounds__(kCombineThreads) attention_paged_combine_kerne
         if (lse[i] == -INFINITY) continue;
         const float w = ex2_approx(lse[i] - m);
         sum += w;
-        acc[0] = fmaf(w, x[i][0].x, acc[0]);
-        acc[1] = fmaf(w, x[i][0].y, acc[1]);
-        acc[2] = fmaf(w, x[i][0].z, acc[2]);
-        acc[3] = fmaf(w, x[i][0].w, acc[3]);
-        acc[4] = fmaf(w, x[i][1].x, acc[4]);
-        acc[5] = fmaf(w, x[i][1].y, acc[5]);
-        acc[6] = fmaf(w, x[i][1].z, acc[6]);
-        acc[7] = fmaf(w, x[i][1].w, acc[7]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          acc[4 * v + 0] = fmaf(w, x[i][v].x, acc[4 * v + 0]);
+          acc[4 * v + 1] = fmaf(w, x[i][v].y, acc[4 * v + 1]);
+          acc[4 * v + 2] = fmaf(w, x[i][v].z, acc[4 * v + 2]);
+          acc[4 * v + 3] = fmaf(w, x[i][v].w, acc[4 * v + 3]);
+        }
       }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    uint4 o;
-    o.x = pack_half2(acc[0] * inv, acc[1] * inv);
-    o.y = pack_half2(acc[2] * inv, acc[3] * inv);
-    o.z = pack_half2(acc[4] * inv, acc[5] * inv);
-    o.w = pack_half2(acc[6] * inv, acc[7] * inv);
-    *reinterpret_cast<uint4*>(a.O + tok * a.ldo +
-                              ((long long)h * a.group + pr - (long long)tok * a.group) * D + v0 * 4) = o;
+    uint32_t o[2 * V];
+#pragma unroll
+    for (int e = 0; e < 2 * V; ++e) o[e] = pack_half2(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    __half* to = a.O + tok * a.ldo +
+                 ((long long)h * a.group + pr - (long long)tok * a.group) * D + v0 * 4;
+    if constexpr (V == 1) *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
+    else *reinterpret_cast<uint4*>(to) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -246,6 +246,7 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
       rows = std::max(rows, std::min<int64_t>((int64_t)a.total_q * a.group, kNarrowRows));
     const int nr = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     n.unit_tok = nr / a.group;
+    n.unit_cost = kNarrowUnitCost;
     n.requests_here = 1;
     n.prefix_here = narrow_prefix;
     const auto kernel = nr == 4   ? attention_paged_narrow_kernel<D, 4>
@@ -255,10 +256,13 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
                    NarrowSmem<D>::kAlloc, stream, "paged attention launch", tmK, tmV, n);
     if (s != HXB_OK) return s;
   }
-  const int64_t chunks = ((int64_t)a.total_q * a.group + 31) / 32;
-  const int col_blocks = chunks * a.kv_heads >= 4 * dev.num_sms ? 1 : D / kCombineCols;
-  return launch_pdl(attention_paged_combine_kernel<D>,
-                    dim3((unsigned)chunks, (unsigned)(a.kv_heads * col_blocks)),
+  // few rows: many blocks of few columns, to have the partials of a row in flight
+  // at once; many: all columns in a block, so that rows without work are few blocks
+  const int64_t chunks = ((int64_t)a.total_q * a.group + 31) / 32, units = chunks * a.kv_heads;
+  const bool few = 2 * units < dev.num_sms;
+  const int col_blocks = units >= 4 * dev.num_sms ? 1 : D / (few ? 16 : 32);
+  const auto combine = few ? attention_paged_combine_kernel<D, 1> : attention_paged_combine_kernel<D, 2>;
+  return launch_pdl(combine, dim3((unsigned)chunks, (unsigned)(a.kv_heads * col_blocks)),
                     dim3(kCombineThreads), 0, stream, "paged attention combine launch", a);
 }
 
@@ -298,7 +302,7 @@ extern "C" hxb_status_t hxb_attention_paged_f16(const hxb_attention_paged_t* arg
   if (group > kBM)
     return fail(HXB_STATUS_UNSUPPORTED, "paged attention: %lld query heads per KV head (at most %d)",
                 (long long)group, kBM);
-  if (kv_heads * (head_dim / kCombineCols) > 65535 || total_q > INT32_MAX / q_heads || table_cols < 1 || table_ld < table_cols ||
+  if (kv_heads * (head_dim / 16) > 65535 || total_q > INT32_MAX / q_heads || table_cols < 1 || table_ld < table_cols ||
       table_cols > INT32_MAX / 2 / block_rows || prefix_len < 0 || prefix_len > INT32_MAX / 2)
     return fail(HXB_STATUS_INVALID_ARGUMENT, "paged attention: bad extents");
   if (!(scale > 0.0f) || !isfinite(scale))
