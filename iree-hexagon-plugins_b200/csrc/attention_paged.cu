@@ -32,9 +32,16 @@
 namespace hxb {
 namespace {
 
-// A prefix that at most this many rows per KV head share goes to the narrow
-// kernel, which reads it once per 16 rows (from L2 after the first).
-constexpr int kNarrowPrefixRows = 64;
+// Whether a prefix of `blocks` key blocks that `rows` rows per KV head share goes
+// to the narrow kernel, beside the requests' own keys. It reads the prefix once
+// per 16 rows (from L2 after the first), 0.85 us a block and SM; a launch of the
+// wide kernel for it costs 12 us, then 2.05 us per 256 rows or 1.4 for the last
+// 128 (one B200, D = 128).
+bool prefix_to_narrow(int64_t rows, int64_t blocks, int64_t kv_heads, int num_sms) {
+  const double narrow = (double)((rows + 15) / 16) * 0.85;
+  const double wide = rows <= 128 ? 1.4 : (double)((rows + 255) / 256) * 2.05;
+  return (narrow - wide) * (double)(blocks * kv_heads) <= 12.0 * num_sms;
+}
 
 // What a row unit costs on top of its key blocks (Q, the first softmax without an
 // overlapping product, the epilogue), in blocks.
@@ -226,7 +233,8 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   const bool narrow = narrow_tok > 0 && max_q_len <= narrow_tok;
   const bool prefix = a.prefix_len > 0;
   const bool narrow_prefix =
-      narrow && prefix && (int64_t)a.total_q * a.group <= kNarrowPrefixRows;
+      narrow && prefix && prefix_to_narrow((int64_t)a.total_q * a.group,
+                                           (a.prefix_len + kBN - 1) / kBN, a.kv_heads, dev.num_sms);
   if (!narrow || (prefix && !narrow_prefix)) {
     PagedArgs w = a;
     w.unit_tok = 2 * a.tile_tok;

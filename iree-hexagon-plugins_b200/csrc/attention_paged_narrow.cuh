@@ -458,12 +458,13 @@ __global__ void __launch_bounds__(kNarThreads, 2)
         if (key_vote(need || bad)) {
           // the block maximum of every row over the 128 keys
           float* rd = red + (blocks_done & 1) * 64;
-          float mx[NR];
 #pragma unroll
-          for (int q = 0; q < NR; ++q) mx[q] = warp_max(x[q]);
-          if (lane == 0)
-#pragma unroll
-            for (int q = 0; q < NR; ++q) rd[quarter * 16 + q] = mx[q];
+          for (int g = 0; g < NR; g += 4) {
+            if (g >= rows) break;  // (uniform)
+            const float4 mx = make_float4(warp_max(x[g]), warp_max(x[g + 1]), warp_max(x[g + 2]),
+                                          warp_max(x[g + 3]));
+            if (lane == 0) *reinterpret_cast<float4*>(rd + quarter * 16 + g) = mx;
+          }
           // O^T of the block before is complete
           if (j > 0) wait(p_done, (blocks_done & 1) ^ 1);
           if (key_vote(bad)) { stop = true; break; }
@@ -475,6 +476,7 @@ __global__ void __launch_bounds__(kNarThreads, 2)
           }
 #pragma unroll
           for (int q = 0; q < NR; ++q) {
+            if (q % 4 == 0 && q >= rows) break;  // (uniform)
             const float m_new =
                 fmaxf(m_run[q], fmaxf(fmaxf(rd[q], rd[16 + q]), fmaxf(rd[32 + q], rd[48 + q])));
             const float alpha = m_run[q] == -INFINITY ? 0.0f : ex2_approx(m_run[q] - m_new);
@@ -491,6 +493,7 @@ __global__ void __launch_bounds__(kNarThreads, 2)
         if (blocks_done > 0) wait(p_done, (blocks_done & 1) ^ 1);
 #pragma unroll
         for (int q = 0; q < NR; ++q) {
+          if (q % 4 == 0 && q >= rows) break;  // (uniform)
           const float pv = ex2_approx(x[q] - (m_run[q] == -INFINITY ? 0.0f : m_run[q]));
           l_part[q] += pv;
           *reinterpret_cast<__half*>(p_smem + q * 128 + ((p_chunk ^ (q & 7)) << 4) + p_in) =
