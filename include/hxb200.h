@@ -480,41 +480,52 @@ hxb_status_t hxb_decoder_block_w8a16_cached(const hxb_decoder_w8_t* w,
  * reached are unspecified. */
 
 /* The tables of one step, for requests with cached_lens[b] rows in the cache
- * and new_lens[b] tokens to add (batch <= 16384, block_rows >= 1):
- *   q_start  [batch + 1]   first row of each request among the step's tokens
- *   kv_lens  [batch]       cached_lens + new_lens; may be cached_lens itself
- *   block_table            entries of the blocks a request begins in this step
- *                          are taken from free_blocks[*cursor ..] in request
- *                          order; the other entries are left as they are
- *   slots    [max_tokens]  block * block_rows + row of each new token, -1
- *                          behind the last one
- *   cursor_out [2]         the cursor behind the blocks taken (may be cursor),
- *                          then how many blocks the free list was short of:
- *                          tokens without a block get slot -1 and table entry
- *                          -1
- * A request is cut at table_cols * block_rows rows, the batch at max_tokens
- * tokens (both set HXB_DEVICE_STATUS_BAD_INDEX). No other output may overlap
- * an input. */
-hxb_status_t hxb_paged_tables(const int32_t* cached_lens, const int32_t* new_lens,
-                              int64_t batch, int64_t block_rows,
-                              const int32_t* free_blocks, int64_t num_free,
-                              const int32_t* cursor, int32_t* block_table,
-                              int64_t table_ld, int64_t table_cols,
-                              int32_t* q_start, int32_t* kv_lens, int64_t* slots,
-                              int64_t max_tokens, int32_t* cursor_out, void* stream);
+ * and new_lens[b] tokens to add. Block table entries of the blocks a request
+ * begins in this step are taken from free_blocks[*cursor ..] in request order;
+ * the other entries are left as they are. A request is cut at table_cols *
+ * block_rows rows, the batch at max_tokens tokens (both set
+ * HXB_DEVICE_STATUS_BAD_INDEX). */
+typedef struct hxb_paged_tables_s {
+  const int32_t* cached_lens; /* [batch], batch <= 16384 */
+  const int32_t* new_lens;    /* [batch] */
+  int64_t batch;
+  int64_t block_rows;         /* rows per block, any number >= 1 */
+  const int32_t* free_blocks; /* [num_free] block ids */
+  int64_t num_free;
+  const int32_t* cursor;      /* [1] first free block not yet taken */
+  int32_t* block_table;       /* [batch, table_ld], table_cols of them used */
+  int64_t table_ld, table_cols;
+  int32_t* q_start;           /* [batch + 1] first row of each request among the */
+                              /* step's tokens */
+  int32_t* kv_lens;           /* [batch] cached + new; may be cached_lens itself */
+  int64_t* slots;             /* [max_tokens] block * block_rows + row of each new */
+  int64_t max_tokens;         /* token, -1 behind the last one */
+  int32_t* cursor_out;        /* [2] the cursor behind the blocks taken (may be */
+                              /* cursor itself), then how many blocks the free */
+                              /* list was short of: tokens without a block get */
+                              /* slot -1 and table entry -1 */
+} hxb_paged_tables_t;         /* (no other output may overlap an input) */
+
+hxb_status_t hxb_paged_tables(const hxb_paged_tables_t* args, void* stream);
 
 /* hxb_kv_cache_write_f16 through a slot map:
  *   k_cache[slots[t] / block_rows, h, slots[t] % block_rows, :] =
  *       k_src[t, h*D : (h+1)*D]
- * and V alike, for t < tokens. Sources are row-major [tokens, ld_src] f16 with
- * 16-byte aligned rows. A negative slot writes nothing (padded rows); equal
- * slots leave either row. head_dim is a multiple of 8. */
-hxb_status_t hxb_kv_cache_write_paged_f16(const void* k_src, const void* v_src,
-                                          int64_t ld_src, const int64_t* slots,
-                                          int64_t tokens, void* k_cache, void* v_cache,
-                                          int64_t block_stride, int64_t num_blocks,
-                                          int64_t kv_heads, int64_t block_rows,
-                                          int64_t head_dim, void* stream);
+ * and V alike, for t < tokens. A negative slot writes nothing (padded rows);
+ * equal slots leave either row. */
+typedef struct hxb_kv_cache_write_paged_s {
+  const void* k_src; /* f16 [tokens, kv_heads * head_dim], rows ld_src apart, */
+  const void* v_src; /* 16-byte aligned */
+  int64_t ld_src;
+  const int64_t* slots; /* [tokens] */
+  int64_t tokens;
+  void* k_cache;
+  void* v_cache;
+  int64_t block_stride, num_blocks, kv_heads, block_rows;
+  int64_t head_dim; /* a multiple of 8, at most 1024 */
+} hxb_kv_cache_write_paged_t;
+
+hxb_status_t hxb_kv_cache_write_paged_f16(const hxb_kv_cache_write_paged_t* args, void* stream);
 
 /* Grouped-query attention of a batch over a paged cache, behind a prefix that
  * all its requests share and that is read once for all of them. Rows

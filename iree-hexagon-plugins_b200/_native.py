@@ -75,10 +75,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                        c_i64, c_i64, c_vp]),
     "hxb_decoder_block_w8a16": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
                                         c_size, c_vp]),
-    "hxb_paged_tables": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,
-                                 c_vp, c_vp, c_vp, c_i64, c_vp, c_vp]),
-    "hxb_kv_cache_write_paged_f16": (c_int, [c_vp, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
-                                             c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "hxb_paged_tables": (c_int, [c_vp, c_vp]),
+    "hxb_kv_cache_write_paged_f16": (c_int, [c_vp, c_vp]),
     "hxb_attention_paged_f16": (c_int, [c_vp, c_vp]),
     "hxb_attention_paged_workspace_bytes": (c_size, [c_i64, c_i64, c_i64, c_i64]),
     # include/hxb200_hal.h: executable library
@@ -275,6 +273,24 @@ class DecoderW8(ctypes.Structure):
                 ("w_o", c_vp), ("s_o", c_vp), ("ffn_norm", c_vp),
                 ("w_gate_up", c_vp), ("s_gate_up", c_vp),
                 ("w_down", c_vp), ("s_down", c_vp)]
+
+
+class PagedTables(ctypes.Structure):
+    """hxb_paged_tables_t of include/hxb200.h."""
+
+    _fields_ = [("cached_lens", c_vp), ("new_lens", c_vp), ("batch", c_i64), ("block_rows", c_i64),
+                ("free_blocks", c_vp), ("num_free", c_i64), ("cursor", c_vp), ("block_table", c_vp),
+                ("table_ld", c_i64), ("table_cols", c_i64), ("q_start", c_vp), ("kv_lens", c_vp),
+                ("slots", c_vp), ("max_tokens", c_i64), ("cursor_out", c_vp)]
+
+
+class KvCacheWritePaged(ctypes.Structure):
+    """hxb_kv_cache_write_paged_t of include/hxb200.h."""
+
+    _fields_ = [("k_src", c_vp), ("v_src", c_vp), ("ld_src", c_i64), ("slots", c_vp),
+                ("tokens", c_i64), ("k_cache", c_vp), ("v_cache", c_vp), ("block_stride", c_i64),
+                ("num_blocks", c_i64), ("kv_heads", c_i64), ("block_rows", c_i64),
+                ("head_dim", c_i64)]
 
 
 class AttentionPaged(ctypes.Structure):

@@ -255,14 +255,11 @@ hxb_status_t check_paged_cache(const char* what, const void* k_cache, const void
 
 using hxb::fail;
 
-extern "C" hxb_status_t hxb_paged_tables(const int32_t* cached_lens, const int32_t* new_lens,
-                                         int64_t batch, int64_t block_rows,
-                                         const int32_t* free_blocks, int64_t num_free,
-                                         const int32_t* cursor, int32_t* block_table,
-                                         int64_t table_ld, int64_t table_cols, int32_t* q_start,
-                                         int32_t* kv_lens, int64_t* slots, int64_t max_tokens,
-                                         int32_t* cursor_out, void* stream) {
+extern "C" hxb_status_t hxb_paged_tables(const hxb_paged_tables_t* args, void* stream) {
   using namespace hxb;
+  if (!args) return fail(HXB_STATUS_INVALID_ARGUMENT, "paged_tables: null arguments");
+  const auto& [cached_lens, new_lens, batch, block_rows, free_blocks, num_free, cursor, block_table,
+               table_ld, table_cols, q_start, kv_lens, slots, max_tokens, cursor_out] = *args;
   if (batch < 1 || batch > kTabMaxBatch)
     return fail(HXB_STATUS_INVALID_ARGUMENT, "paged_tables: 1 to %d requests, not %lld",
                 kTabMaxBatch, (long long)batch);
@@ -328,11 +325,12 @@ extern "C" hxb_status_t hxb_paged_tables(const int32_t* cached_lens, const int32
   return cuda_status(cudaLaunchKernelEx(&cfg, paged_tables_kernel, a), "paged tables launch");
 }
 
-extern "C" hxb_status_t hxb_kv_cache_write_paged_f16(
-    const void* k_src, const void* v_src, int64_t ld_src, const int64_t* slots, int64_t tokens,
-    void* k_cache, void* v_cache, int64_t block_stride, int64_t num_blocks, int64_t kv_heads,
-    int64_t block_rows, int64_t head_dim, void* stream) {
+extern "C" hxb_status_t hxb_kv_cache_write_paged_f16(const hxb_kv_cache_write_paged_t* args,
+                                                     void* stream) {
   using namespace hxb;
+  if (!args) return fail(HXB_STATUS_INVALID_ARGUMENT, "paged cache write: null arguments");
+  const auto& [k_src, v_src, ld_src, slots, tokens, k_cache, v_cache, block_stride, num_blocks,
+               kv_heads, block_rows, head_dim] = *args;
   hxb_status_t s = check_paged_cache("paged cache write", k_cache, v_cache, block_stride,
                                      num_blocks, kv_heads, block_rows, head_dim);
   if (s != HXB_OK) return s;

@@ -25,9 +25,11 @@ import torch
 from . import _native
 from ._native import check
 
-# hxb_attention_paged_t: packing the record is several times cheaper than
-# converting its 26 fields one by one.
-_ARGUMENTS = struct.Struct("=QqQqQQqqqQQqqqQqqQqqqqfiQQ")
+# The entries' argument records (the structures of _native): packing one is
+# several times cheaper than converting its fields one by one.
+_TABLES = struct.Struct("=QQqqQqQQqqQQQqQ")
+_WRITE = struct.Struct("=QQqQqQQqqqqq")
+_ATTENTION = struct.Struct("=QqQqQQqqqQQqqqQqqQqqqqfiQQ")
 _NO_GUARD = contextlib.nullcontext()
 _I32, _I64, _F16 = torch.int32, torch.int64, torch.float16
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -110,14 +112,14 @@ def paged_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks:
         cursor_out = cached_lens.new_empty(2)
     table_p, ld, cols = _table(block_table, B, index)
     with _on(cached_lens.device):
-        check(lib.hxb_paged_tables(
+        check(lib.hxb_paged_tables(_TABLES.pack(
             _ints("cached_lens", cached_lens, _I32, B, index),
             _ints("new_lens", new_lens, _I32, B, index), B, block_rows,
             _ints("free_blocks", free_blocks, _I32, 0, index), free_blocks.numel(),
             _ints("cursor", cursor, _I32, 1, index), table_p, ld, cols,
             _ints("q_start", q_start, _I32, B + 1, index), _ints("kv_lens", kv_lens, _I32, B, index),
             _ints("slots", slots, _I64, n, index), n,
-            _ints("cursor_out", cursor_out, _I32, 2, index), _raw_stream(index)))
+            _ints("cursor_out", cursor_out, _I32, 2, index)), _raw_stream(index)))
     return q_start, kv_lens, slots, cursor_out
 
 
@@ -138,10 +140,10 @@ def kv_cache_write_paged(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torc
         raise ValueError("sources and caches must share a device")
     n = shape[0]
     with _on(k_cache.device):
-        check(lib.hxb_kv_cache_write_paged_f16(
+        check(lib.hxb_kv_cache_write_paged_f16(_WRITE.pack(
             k_src.data_ptr(), v_src.data_ptr(), src_stride[0] if n > 1 else heads * D,
             _ints("slots", slots, _I64, n, index), n, k_cache.data_ptr(), v_cache.data_ptr(), stride,
-            blocks, heads, rows, D, _raw_stream(index)))
+            blocks, heads, rows, D), _raw_stream(index)))
 
 
 @functools.lru_cache(maxsize=256)
@@ -208,7 +210,7 @@ def attention_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
             if workspace.get_device() != index or not workspace.is_contiguous():
                 raise ValueError("workspace must be a contiguous buffer on the caches' device")
             nbytes = workspace.numel() * workspace.element_size()
-        check(lib.hxb_attention_paged_f16(_ARGUMENTS.pack(
+        check(lib.hxb_attention_paged_f16(_ATTENTION.pack(
             query.data_ptr(), q_stride[0] if n > 1 else row, out.data_ptr(),
             o_stride[0] if n > 1 else row, _ints("q_start", q_start, _I32, B + 1, index),
             _ints("kv_lens", kv_lens, _I32, B, index), B, n,

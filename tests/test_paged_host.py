@@ -15,10 +15,7 @@ def attention(pkg, **kw):
         v_cache=A, block_stride=2 * 16 * 128, num_blocks=8, block_rows=16, block_table=A, table_ld=4,
         table_cols=4, prefix_table=A, prefix_len=20, q_heads=8, kv_heads=2, head_dim=128, scale=0.1,
         causal=1, workspace=A, workspace_bytes=1 << 40)
-    for name, value in kw.items():
-        assert hasattr(a, name)
-        setattr(a, name, value)
-    return pkg._native.load().hxb_attention_paged_f16(ctypes.byref(a), None)
+    return pkg._native.load().hxb_attention_paged_f16(filled(a, kw), None)
 
 
 @pytest.mark.parametrize("kw,status,text", [
@@ -62,56 +59,67 @@ def test_attention_paged_without_tokens_is_nothing(pkg):
     assert attention(pkg, total_q=0, q=None, out=None, workspace=None, workspace_bytes=0) == 0
 
 
-def test_attention_paged_arguments_have_the_layout_of_the_wrapper(pkg):
-    """The Python entry packs the argument record by itself."""
-    native = pkg._native.AttentionPaged
-    assert pkg.paged._ARGUMENTS.size == ctypes.sizeof(native)
-    values = list(range(1, 23)) + [0.5, 24, 25, 26]
-    got = native.from_buffer_copy(pkg.paged._ARGUMENTS.pack(*values))
-    assert [getattr(got, f[0]) for f in native._fields_] == values
-    assert pkg._native.load().hxb_attention_paged_f16(None, None) == 1
+@pytest.mark.parametrize("packed,structure,entry", [
+    ("_TABLES", "PagedTables", "hxb_paged_tables"),
+    ("_WRITE", "KvCacheWritePaged", "hxb_kv_cache_write_paged_f16"),
+    ("_ATTENTION", "AttentionPaged", "hxb_attention_paged_f16"),
+])
+def test_argument_records_have_the_layout_of_the_wrappers(pkg, packed, structure, entry):
+    """The Python entries pack the argument records by themselves."""
+    packed, structure = getattr(pkg.paged, packed), getattr(pkg._native, structure)
+    assert packed.size == ctypes.sizeof(structure)
+    values = [0.5 if f[0] == "scale" else i + 1 for i, f in enumerate(structure._fields_)]
+    got = structure.from_buffer_copy(packed.pack(*values))
+    assert [getattr(got, f[0]) for f in structure._fields_] == values
+    assert getattr(pkg._native.load(), entry)(None, None) == 1
 
 
-def tables(lib, **kw):
-    a = dict(cached=A, new=A, batch=2, rows=16, free=A, num_free=4, cursor=A, table=A, table_ld=4,
-             cols=4, q_start=A, kv_lens=A, slots=A, max_tokens=8, cursor_out=A, stream=None)
-    assert set(kw) <= set(a)
-    a.update(kw)
-    return lib.hxb_paged_tables(*a.values())
+def filled(structure, kw):
+    for name, value in kw.items():
+        assert hasattr(structure, name)
+        setattr(structure, name, value)
+    return ctypes.byref(structure)
+
+
+def tables(pkg, **kw):
+    a = pkg._native.PagedTables(
+        cached_lens=A, new_lens=A, batch=2, block_rows=16, free_blocks=A, num_free=4, cursor=A,
+        block_table=A, table_ld=4, table_cols=4, q_start=A, kv_lens=A, slots=A, max_tokens=8,
+        cursor_out=A)
+    return pkg._native.load().hxb_paged_tables(filled(a, kw), None)
 
 
 @pytest.mark.parametrize("kw,text", [
-    (dict(batch=0), b"requests"), (dict(batch=16385), b"requests"), (dict(rows=0), b"extents"),
-    (dict(cols=0), b"extents"), (dict(cols=5), b"extents"), (dict(max_tokens=-1), b"extents"),
-    (dict(num_free=-1), b"extents"), (dict(rows=1 << 20, cols=1 << 12, table_ld=1 << 12), b"extents"),
-    (dict(cached=None), b"null"), (dict(free=None), b"null"), (dict(slots=None), b"null"),
+    (dict(batch=0), b"requests"), (dict(batch=16385), b"requests"), (dict(block_rows=0), b"extents"),
+    (dict(table_cols=0), b"extents"), (dict(table_cols=5), b"extents"),
+    (dict(max_tokens=-1), b"extents"), (dict(num_free=-1), b"extents"),
+    (dict(block_rows=1 << 20, table_cols=1 << 12, table_ld=1 << 12), b"extents"),
+    (dict(cached_lens=None), b"null"), (dict(free_blocks=None), b"null"), (dict(slots=None), b"null"),
     (dict(cursor_out=None), b"null"),
 ])
 def test_paged_tables_refuses(pkg, kw, text):
-    lib = pkg._native.load()
-    assert tables(lib, **kw) == 1
-    assert text in lib.hxb_last_error_message()
+    assert tables(pkg, **kw) == 1
+    assert text in pkg._native.load().hxb_last_error_message()
 
 
-def write(lib, **kw):
-    a = dict(k=A, v=A, ld=256, slots=A, tokens=3, kc=A, vc=A, stride=2 * 16 * 128, blocks=8, heads=2,
-             rows=16, D=128, stream=None)
-    assert set(kw) <= set(a)
-    a.update(kw)
-    return lib.hxb_kv_cache_write_paged_f16(*a.values())
+def write(pkg, **kw):
+    a = pkg._native.KvCacheWritePaged(
+        k_src=A, v_src=A, ld_src=256, slots=A, tokens=3, k_cache=A, v_cache=A,
+        block_stride=2 * 16 * 128, num_blocks=8, kv_heads=2, block_rows=16, head_dim=128)
+    return pkg._native.load().hxb_kv_cache_write_paged_f16(filled(a, kw), None)
 
 
 @pytest.mark.parametrize("kw,status,text", [
-    (dict(rows=24), 2, b"power of two"), (dict(D=12), 2, b"head_dim"), (dict(D=2048), 2, b"head_dim"),
-    (dict(tokens=-1), 1, b"token count"), (dict(k=None), 1, b"null"), (dict(slots=None), 1, b"null"),
-    (dict(ld=255), 1, b"16-byte"), (dict(ld=248), 1, b"16-byte"), (dict(v=A + 8), 1, b"16-byte"),
-    (dict(kc=A + 8), 1, b"16-byte"), (dict(stride=128), 1, b"block_stride"),
-    (dict(heads=0), 1, b"cache extents"),
+    (dict(block_rows=24), 2, b"power of two"), (dict(head_dim=12), 2, b"head_dim"),
+    (dict(head_dim=2048), 2, b"head_dim"), (dict(tokens=-1), 1, b"token count"),
+    (dict(k_src=None), 1, b"null"), (dict(slots=None), 1, b"null"),
+    (dict(ld_src=255), 1, b"16-byte"), (dict(ld_src=248), 1, b"16-byte"),
+    (dict(v_src=A + 8), 1, b"16-byte"), (dict(k_cache=A + 8), 1, b"16-byte"),
+    (dict(block_stride=128), 1, b"block_stride"), (dict(kv_heads=0), 1, b"cache extents"),
 ])
 def test_kv_cache_write_paged_refuses(pkg, kw, status, text):
-    lib = pkg._native.load()
-    assert write(lib, **kw) == status
-    assert text in lib.hxb_last_error_message()
+    assert write(pkg, **kw) == status
+    assert text in pkg._native.load().hxb_last_error_message()
 
 
 def test_workspace_query_of_invalid_extents_is_zero(pkg):
