@@ -511,8 +511,8 @@ hxb_status_t hxb_paged_tables(const hxb_paged_tables_t* args, void* stream);
 /* hxb_kv_cache_write_f16 through a slot map:
  *   k_cache[slots[t] / block_rows, h, slots[t] % block_rows, :] =
  *       k_src[t, h*D : (h+1)*D]
- * and V alike, for t < tokens. A negative slot writes nothing (padded rows);
- * equal slots leave either row. */
+ * and V alike, for t < tokens. A negative slot writes nothing (padded rows); the
+ * others must differ (what equal slots leave is unspecified). */
 typedef struct hxb_kv_cache_write_paged_s {
   const void* k_src; /* f16 [tokens, kv_heads * head_dim], rows ld_src apart, */
   const void* v_src; /* 16-byte aligned */
@@ -538,7 +538,7 @@ hxb_status_t hxb_kv_cache_write_paged_f16(const hxb_kv_cache_write_paged_t* args
  * Query head h reads KV head h / (q_heads / kv_heads), at most 128 query heads
  * per KV head; head_dim 64 or 128. prefix_len 0 runs without a prefix. Tokens
  * that see no key are 0; rows of out before q_start[0] and from
- * q_start[batch] on are left as they are. Cache rows behind a length are not
+ * q_start[batch] on are left as they are. out must not overlap an input. Cache rows behind a length are not
  * used, whatever they hold; rows within it must be finite where a token of
  * the request may not see them. f32 scores, statistics and sums; P is rounded
  * to f16 for the second product. A call of more than 2^30 pairs of a query

@@ -14,9 +14,9 @@
 // (attention_paged_narrow.cuh, keys on the TMEM lanes, bound by HBM) takes the
 // own keys of decode batches, at most 16 rows per KV head and request, the wide
 // one (attention_paged_wide.cuh, rows on the lanes, bound by the tensor core)
-// those of other batches and a prefix that many rows share. A combine kernel merges what each row has. K and V blocks come
-// through 3-D tensor maps, one TMA box per cache block and 64 columns, straight
-// into the 128B-swizzled tile.
+// those of other batches and a prefix that many rows share. A combine kernel
+// merges what each row has. K and V blocks come through 3-D tensor maps, one TMA
+// box per cache block and 64 columns, straight into the 128B-swizzled tile.
 //
 // The reference's KV-cache models attend one contiguous cache with one length
 // for the batch (integration_tests/models/kv_cache.py:46-112); the shared
@@ -310,8 +310,8 @@ extern "C" hxb_status_t hxb_attention_paged_f16(const hxb_attention_paged_t* arg
   if (group > kBM)
     return fail(HXB_STATUS_UNSUPPORTED, "paged attention: %lld query heads per KV head (at most %d)",
                 (long long)group, kBM);
-  if (kv_heads * (head_dim / 16) > 65535 || total_q > INT32_MAX / q_heads || table_cols < 1 || table_ld < table_cols ||
-      table_cols > INT32_MAX / 2 / block_rows || prefix_len < 0 || prefix_len > INT32_MAX / 2)
+  if (kv_heads * (head_dim / 16) > 65535 || total_q > INT32_MAX / q_heads || table_cols < 1 ||
+      table_ld < table_cols || table_cols > INT32_MAX / 2 / block_rows || prefix_len < 0 || prefix_len > INT32_MAX / 2)
     return fail(HXB_STATUS_INVALID_ARGUMENT, "paged attention: bad extents");
   if (!(scale > 0.0f) || !isfinite(scale))
     return fail(HXB_STATUS_INVALID_ARGUMENT, "paged attention: scale must be finite and > 0");

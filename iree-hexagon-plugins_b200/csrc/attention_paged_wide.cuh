@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the answer before its PV, so both barriers keep in step; a job of -1
       // is the end.
       uint32_t fixes = 0;
-      while (__all_sync(0xffffffffu, mbar_wait(v_need, fixes++ & 1, fs))) {
+      while (__all_sync(0xffffffffu, mbar_wait_for(v_need, fixes++ & 1, fs, kLongWaitNs))) {
         const int job = *v_job;
         if (job < 0) break;
         uint8_t* tile = smem + L::kOffKV + (job >> 8) * kTileBytes;

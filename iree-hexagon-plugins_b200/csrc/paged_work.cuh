@@ -8,10 +8,10 @@
 // itself (prompt chunks), sharing the prefix would only add partial results: then
 // each request's segment visits the prefix blocks first and its own after them.
 // All of that is laid end to end in units of one block (a row unit counts
-// unit_cost more for its start and end) -- prefix, request 0, request 1 ...; inside a segment KV
-// head by KV head, row unit by row unit -- and CTA i takes units [i S, (i + 1) S),
-// S = ceil(T / CTAs): equal shares whatever the lengths, which are read on the
-// GPU. The part of a row unit's blocks that falls to one CTA is an item;
+// unit_cost more for its start and end) -- prefix, request 0, request 1 ...;
+// inside a segment KV head by KV head, row unit by row unit -- and CTA i takes
+// units [i S, (i + 1) S), S = ceil(T / CTAs): equal shares whatever the lengths,
+// which are read on the GPU. The part of a row unit's blocks that falls to one CTA is an item;
 // a row unit cut between CTAs leaves one partial result per CTA.
 #pragma once
 
@@ -215,6 +215,7 @@ struct ShareSmem {
 // the whole block.
 template <int THREADS>
 __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREADS>& sm) {
+  if (threadIdx.x == 0) sm.seg.work = 0;  // (no segment, until its thread notes one)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int each = a.requests_here ? (a.batch + THREADS - 1) / THREADS : 0;
   const int b0 = min((int)threadIdx.x * each, a.batch), b1 = min(b0 + each, a.batch);
@@ -300,6 +301,11 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const F
   return wait_slow(bar, parity, fs.abort, fs.status);
 }
 
+// Limit of a wait that a correct call may spend a large part of its time in (for a
+// tile to zero, for a long item's end): a launch that is stuck ends by the limit of
+// another role's wait, whose flag these waits watch.
+constexpr unsigned long long kLongWaitNs = 32 * kWaitLimitNs;
+
 // Publishes the CTA's items, one after the other, into a ring of N records (one
 // thread). item_empty[] collects one arrival of every reader of a record.
 // OUT_OF_LINE: wait through wait_bar (not in a kernel that moves registers with
@@ -373,7 +379,9 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
     }
     uint64_t* free_slot = &item_empty[out.slot()];
     const uint32_t parity = out.parity() ^ 1;
-    if (!(OUT_OF_LINE ? wait_bar(free_slot, parity, fs) : mbar_wait(free_slot, parity, fs))) return;
+    if (!(OUT_OF_LINE ? wait_bar(free_slot, parity, fs)
+                      : mbar_wait_for(free_slot, parity, fs, kLongWaitNs)))
+      return;
     items[out.slot()] = item;
     mbar_arrive(&item_full[out.slot()]);
     ++out.n;

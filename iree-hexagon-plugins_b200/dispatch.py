@@ -343,7 +343,8 @@ def kv_cache_write(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torch.Tens
 
 
 def device_status(clear: bool = True) -> int:
-    """Status bits kernels raised on the current device (1 = a wait timed out)."""
+    """Status bits kernels raised on the current device (1 = a wait timed out,
+    2 = a block number, slot or length lay outside its buffer)."""
     import ctypes
     bits = ctypes.c_int(0)
     check(_native.load().hxb_device_status(int(clear), ctypes.byref(bits)))

@@ -126,9 +126,10 @@ def paged_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks:
 def kv_cache_write_paged(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torch.Tensor,
                          v_cache: torch.Tensor, slots: torch.Tensor) -> None:
     """k_cache[slots[t] // block_rows, h, slots[t] % block_rows] = k_src[t,
-    h*D:(h+1)*D] (and V) for every source row t; a negative slot writes nothing.
-    Sources are [tokens, kv_heads * D] f16 views of one row pitch (e.g. column
-    blocks of a fused QKV output), caches [blocks, kv_heads, block_rows, D]."""
+    h*D:(h+1)*D] (and V) for every source row t; a negative slot writes nothing,
+    the others must differ. Sources are [tokens, kv_heads * D] f16 views of one
+    row pitch (e.g. column blocks of a fused QKV output), caches
+    [blocks, kv_heads, block_rows, D]."""
     lib = _native.load()
     index, blocks, heads, rows, D, stride = _cache(k_cache, v_cache)
     shape, src_stride = k_src.shape, k_src.stride()
@@ -173,8 +174,8 @@ def attention_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     prefix is visible to every token; `causal` makes the tokens of a request its
     last cached rows. `max_q_len` is the most tokens a request is expected to
     have (a hint; by default all of them). Rows of `out` behind q_start[batch]
-    are left as they are. `workspace`: a device buffer of
-    attention_paged_workspace_bytes, allocated here if None."""
+    are left as they are; `out` must not overlap an input. `workspace`: a device
+    buffer of attention_paged_workspace_bytes, allocated here if None."""
     lib = _native.load()
     index, blocks, Hkv, rows, D, stride = _cache(k_cache, v_cache)
     shape, q_stride = query.shape, query.stride()

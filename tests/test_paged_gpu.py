@@ -221,6 +221,61 @@ def test_attention_paged_same_result_every_time(cuda_pkg):
     assert torch.equal(b.run(cuda_pkg, workspace=ws), first)
 
 
+def test_paged_cache_offsets_beyond_32_bits(cuda_pkg):
+    """Blocks 2^31 elements apart: the write lands in them and attention reads them."""
+    Hkv, P, D, far = 2, 16, 128, (1 << 31) + 64
+    block = Hkv * P * D
+    store = torch.empty(2 * far + 2 * block, dtype=torch.float16, device=DEV)
+    k, v = (store[i * block:].as_strided((3, Hkv, P, D), (far, P * D, D, 1)) for i in range(2))
+    g = torch.Generator(device=DEV).manual_seed(1)
+    T, n = 40, 3
+    src = torch.randn(T, 2 * Hkv * D, device=DEV, generator=g).half()
+    slots = torch.cat([torch.arange(16) + 32, torch.arange(16), torch.arange(8) + 16]).to(DEV)
+    cuda_pkg.kv_cache_write_paged(src[:, :Hkv * D], src[:, Hkv * D:], k, v, slots)
+    assert torch.equal(v[2, 1], src[:16, 3 * D:])
+    q = torch.randn(n, 8, D, device=DEV, generator=g).half()
+    for hint in (1, n):  # both kernels
+        got = cuda_pkg.attention_paged(q, k, v, torch.tensor([0, n], **I32), torch.tensor([T - 16], **I32),
+                                       torch.tensor([[0, 1]], **I32), max_q_len=hint,
+                                       prefix_table=torch.tensor([2], **I32), prefix_len=16)
+        kk, vv = src[:, :Hkv * D].double().view(T, Hkv, D), src[:, Hkv * D:].double().view(T, Hkv, D)
+        s = torch.einsum("nhgd,khd->nhgk", q.double().view(n, Hkv, 4, D), kk) * D ** -0.5
+        hidden = torch.arange(T, device=DEV)[None] > T - n + torch.arange(n, device=DEV)[:, None]
+        p = torch.softmax(s.masked_fill(hidden[:, None, None], -math.inf), -1)
+        want = torch.einsum("nhgk,khd->nhgd", p, vv).reshape(n, 8, D)
+        bound = 2 ** -11 * want.abs() + (2 ** -11 + T * 2 ** -25 + 1e-5) * vv.abs().max()
+        assert bool(((got.double() - want).abs() <= bound).all())
+    assert cuda_pkg.device_status() == 0
+
+
+def test_attention_paged_call_of_seconds(cuda_pkg):
+    """A call longer than the limit of one wait of its kernels, with whole key blocks
+    only. Every key set below is the 1024 rows of one cache block over and over, so
+    its softmax is that of the 1024 rows."""
+    n, Hq, Hkv, P, D, times = 16384, 32, 8, 1024, 128, 12000
+    g = torch.Generator(device=DEV).manual_seed(2)
+    k, v = (torch.randn(1, Hkv, P, D, device=DEV, generator=g).half() for _ in range(2))
+    q = torch.randn(n, Hq, D, device=DEV, generator=g).half()
+    table = torch.zeros(1, times, **I32)
+    start, lens = torch.tensor([0, n], **I32), torch.tensor([P * times], **I32)
+    t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t0.record()
+    got = cuda_pkg.attention_paged(q, k, v, start, lens, table, causal=False)
+    t1.record()
+    torch.cuda.synchronize()
+    assert cuda_pkg.device_status() == 0
+    assert t0.elapsed_time(t1) > 2000
+    some = torch.cat([torch.arange(0, n, 997), torch.tensor([n - 1])]).to(DEV)
+    qq = q[some].double().view(-1, Hkv, Hq // Hkv, D)
+    p = torch.softmax(torch.einsum("nhgd,hkd->nhgk", qq, k[0].double()) * D ** -0.5, -1)
+    want = torch.einsum("nhgk,hkd->nhgd", p, v[0].double()).reshape(-1, Hq, D)
+    # P in f16; the sum of a row adds 12000 * 8 blocks' sums in f32, each addition off
+    # by at most 2^-24 of the sum so far, and O the 8 products of each block
+    blocks = times * P // 128
+    bound = 2 ** -11 * want.abs() + (2 ** -11 + (blocks + 8 * blocks) * 2 ** -24) * v.abs().max()
+    assert bool(((got[some].double() - want).abs() <= bound).all())
+
+
 def test_attention_paged_two_streams(cuda_pkg):
     """Calls with workspaces of their own may run at the same time."""
     batches = [Batch([1] * 20, [30 + i * s for i in range(20)], 32, 8, 128, 16, 900, seed=s)
