@@ -293,6 +293,29 @@ def test_attention_paged_two_streams(cuda_pkg):
         assert all(torch.equal(x, w) for x in g)
 
 
+def test_attention_paged_graphs_on_one_workspace(cuda_pkg):
+    """Graphs of both kernels and eager calls take turns on one workspace."""
+    batches = [Batch([1] * 20, [30 + i * s for i in range(20)], 32, 8, 128, 16, p, seed=s)
+               for s, p in ((11, 900), (12, 0))] + [Batch([200, 90], [300, 90], 32, 8, 128, 16, 400)]
+    want = [b.run(cuda_pkg, max_q_len=max(b.new)).clone() for b in batches]
+    nbytes = max(cuda_pkg.attention_paged_workspace_bytes(b.q.shape[0], b.Hq, b.D, b.prefix)
+                 for b in batches)
+    workspace = torch.full((nbytes,), 255, dtype=torch.uint8, device=DEV)
+    graphs, outs = [], []
+    for b in batches:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(b.run(cuda_pkg, max_q_len=max(b.new), workspace=workspace))
+    for i in (0, 1, 2, 1, 0, 2, 2, 0):
+        outs[i].zero_()
+        graphs[i].replay()
+        j = (i + 1) % 3
+        eager = batches[j].run(cuda_pkg, max_q_len=max(batches[j].new), workspace=workspace)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i], want[i]) and torch.equal(eager, want[j])
+    assert cuda_pkg.device_status() == 0
+
+
 def test_attention_paged_bad_indices_are_reported_not_followed(cuda_pkg):
     b = Batch([1, 1], [40, 300], 8, 2, 128, 16, 100, seed=13)
     want = b.run(cuda_pkg).clone()
