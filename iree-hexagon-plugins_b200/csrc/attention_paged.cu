@@ -14,7 +14,9 @@
 // (attention_paged_narrow.cuh, keys on the TMEM lanes, bound by HBM) takes the
 // own keys of decode batches, at most 16 rows per KV head and request, the wide
 // one (attention_paged_wide.cuh, rows on the lanes, bound by the tensor core)
-// those of other batches and a prefix that many rows share. A combine kernel
+// those of other batches and a prefix that many rows share. A decode batch behind
+// a long prefix has both at once, each on its share of the SMs (256 requests of
+// 550 keys behind 4096: 119 us, one kernel after the other 153). A combine kernel
 // merges what each row has. K and V blocks come through 3-D tensor maps, one TMA
 // box per cache block and 64 columns, straight into the 128B-swizzled tile.
 //
@@ -34,13 +36,14 @@ namespace {
 
 // Whether a prefix of `blocks` key blocks that `rows` rows per KV head share goes
 // to the narrow kernel, beside the requests' own keys. It reads the prefix once
-// per 16 rows (from L2 after the first), 0.85 us a block and SM; a launch of the
-// wide kernel for it costs 12 us, then 2.05 us per 256 rows or 1.4 for the last
-// 128 (one B200, D = 128).
+// per 16 rows (from L2 after the first), 0.85 us a block and SM, the wide kernel
+// takes 2.05 us per 256 rows or 1.4 for the last 128; a second kernel costs the call
+// 3 us (one B200, D = 128, 8 KV heads: 64 rows on 16 blocks 23.0 us narrow, 25.9
+// wide; 128 rows on 32 blocks 47.1 us narrow, 35.8 wide, with the step's tables).
 bool prefix_to_narrow(int64_t rows, int64_t blocks, int64_t kv_heads, int num_sms) {
   const double narrow = (double)((rows + 15) / 16) * 0.85;
   const double wide = rows <= 128 ? 1.4 : (double)((rows + 255) / 256) * 2.05;
-  return (narrow - wide) * (double)(blocks * kv_heads) <= 12.0 * num_sms;
+  return (narrow - wide) * (double)(blocks * kv_heads) <= 3.0 * num_sms;
 }
 
 // What a row unit costs on top of its key blocks (Q, the first softmax without an
@@ -235,32 +238,50 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   const bool narrow_prefix =
       narrow && prefix && prefix_to_narrow((int64_t)a.total_q * a.group,
                                            (a.prefix_len + kBN - 1) / kBN, a.kv_heads, dev.num_sms);
-  if (!narrow || (prefix && !narrow_prefix)) {
+  // rows of a unit of the narrow kernel: what the largest request, and a prefix,
+  // can fill
+  int64_t rows = std::max<int64_t>(1, max_q_len) * a.group;
+  if (narrow_prefix) rows = std::max(rows, std::min<int64_t>((int64_t)a.total_q * a.group, kNarrowRows));
+  const int nr = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+  const bool wide = !narrow || (prefix && !narrow_prefix);
+  if (wide) {
     PagedArgs w = a;
     w.unit_tok = 2 * a.tile_tok;
     w.unit_cost = kWideUnitCost;
     w.requests_here = !narrow;
     w.prefix_here = prefix;
     w.fat_tok = !narrow && prefix ? a.tile_tok : 0;
+    w.beside = narrow;
+    w.other_tok = nr / a.group;
+    w.other_cost = kNarrowUnitCost;
     s = launch_pdl(attention_paged_wide_kernel<D>, dim3((unsigned)dev.num_sms), dim3(kThreads),
                    WideSmem<D>::kAlloc, stream, "paged attention launch", tmQ, tmK, tmV, w);
     if (s != HXB_OK) return s;
   }
   if (narrow) {
     PagedArgs n = a;
-    // rows of a unit: what the largest request, and a prefix, can fill
-    int64_t rows = std::max<int64_t>(1, max_q_len) * a.group;
-    if (narrow_prefix)
-      rows = std::max(rows, std::min<int64_t>((int64_t)a.total_q * a.group, kNarrowRows));
-    const int nr = rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
     n.unit_tok = nr / a.group;
     n.unit_cost = kNarrowUnitCost;
     n.requests_here = 1;
     n.prefix_here = narrow_prefix;
+    n.beside = wide;
+    n.other_tok = 2 * a.tile_tok;
+    n.other_cost = kWideUnitCost;
     const auto kernel = nr == 4   ? attention_paged_narrow_kernel<D, 4>
                         : nr == 8 ? attention_paged_narrow_kernel<D, 8>
                                   : attention_paged_narrow_kernel<D, 16>;
-    s = launch_pdl(kernel, dim3((unsigned)(2 * dev.num_sms)), dim3(kNarThreads),
+    int ctas = 2 * dev.num_sms;
+    if (wide) {
+      // Not many more than will have work (the lengths are at most what the table
+      // holds): those that find no SM beside the wide kernel start behind it.
+      const int64_t units = ((int64_t)a.total_q + n.other_tok - 1) / n.other_tok * a.kv_heads;
+      const int64_t work = (a.prefix_len + kBN - 1) / kBN + n.other_cost;
+      const float own = (float)a.kv_heads *
+                        (float)std::min<int64_t>(a.total_q, a.batch + a.total_q / n.unit_tok) *
+                        (float)(((int64_t)a.table_cols << a.rows_log2) / kBN + 1 + n.unit_cost);
+      ctas = ctas_beside(a, (int)units, wide_share(a, (int)units, (int)work, own));
+    }
+    s = launch_pdl(kernel, dim3((unsigned)ctas), dim3(kNarThreads),
                    NarrowSmem<D>::kAlloc, stream, "paged attention launch", tmK, tmV, n);
     if (s != HXB_OK) return s;
   }

@@ -202,8 +202,17 @@ __global__ void __launch_bounds__(kNarThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  pdl_trigger();
-  pdl_wait();
+  // (no pdl_trigger(): combine blocks started early crowd on the SMs that are free
+  // first and merge from there, 1 us of a call of 24, 13 us of one of 66)
+  // Beside the wide kernel: that one has waited for all before it, and started this
+  // one after that, and nothing of it is read here. The fences drop what this SM may
+  // hold of the inputs from before.
+  if (args.beside) {
+    __threadfence();
+    fence_proxy_async_global();
+  } else {
+    pdl_wait();
+  }
   const Share share = find_share(args, share_smem);
 
   // A reader's position in the items (each in shared memory until every reader
@@ -267,7 +276,7 @@ __global__ void __launch_bounds__(kNarThreads, 2)
       const int slot = ring.slot();
       if (!__all_sync(0xffffffffu, wait_bar(&kv_empty[slot], ring.parity() ^ 1, fs))) return false;
       loader.load(args, item.head, which ? &tmV : &tmK, smem + L::kOffKV + slot * kTileBytes,
-                  &kv_full[slot], at.j, id);
+                  &kv_full[slot], at.j, id, item.request >= 0);
       ++ring.n;
       return true;
     });
@@ -582,6 +591,8 @@ __global__ void __launch_bounds__(kNarThreads, 2)
     tc_fence_after();
     tmem_dealloc(tmem_base, kNarTmemCols);
   }
+  // (the combine kernel waits for this one, and so for the wide one)
+  if (args.beside) pdl_wait();
 }
 
 }  // namespace hxb

@@ -125,9 +125,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
-  pdl_trigger();
+  // (in this order: a narrow kernel that runs beside this one does not wait)
   pdl_wait();
+  pdl_trigger();
   const Share share = find_share(args, share_smem);
+  if (share.lo >= share.hi) {  // no work: the SM is the next kernel's
+    if (warp == 1) tmem_dealloc(tmem_base, 512);
+    return;
+  }
 
   // Reads the next item; false at the end and on failure.
   Ring<kItems> it;

@@ -58,6 +58,8 @@ struct PagedArgs {
   int requests_here;       // this kernel takes the requests' own keys
   int prefix_here;         // and the prefix
   int fat_tok;             // requests of so many tokens fill tiles (0: no matter)
+  int beside;              // the other kernel runs at the same time, with
+  int other_tok, other_cost;  // row units of so many tokens and such a cost
   int tile_tok, box_tok;   // wide kernel: tokens per 128-row tile and per Q box
   int table_cols, num_blocks, rows_log2;
   int prefix_len;
@@ -112,6 +114,7 @@ __device__ __forceinline__ int clamp_token(const PagedArgs& a, int b) {
 struct Segment {
   int tok, n, keys;
   int units;       // row units
+  int cost;        // units of work of a row unit's start and end
   int work;        // units of work of one KV head over all row units
   int pre;         // prefix blocks visited before the own ones
   bool causal;
@@ -158,8 +161,8 @@ constexpr int kMostWork = 1 << 30;  // units of work of one call (saturated abov
 __device__ __forceinline__ int work_before(const PagedArgs& a, const Segment& s, int units) {
   if (units == 0) return 0;
   const int last = unit_blocks(a, s, units - 1);  // the most blocks of a unit
-  if ((float)units * (float)(last + a.unit_cost) >= (float)kMostWork) return kMostWork;
-  int sum = units * a.unit_cost + last;
+  if ((float)units * (float)(last + s.cost) >= (float)kMostWork) return kMostWork;
+  int sum = units * s.cost + last;
   if (!s.causal) return sum + (units - 1) * last;
   // unit u < units - 1 sees d + (u + 1) T own keys: none up to u = dark, then one
   // block per begun 128
@@ -182,6 +185,7 @@ __device__ __forceinline__ Segment own_segment(const PagedArgs& a, int b, int pr
   s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
   s.pre = pre;
   s.causal = a.causal != 0;
+  s.cost = a.unit_cost;
   s.work = work_before(a, s, s.units);
   return s;
 }
@@ -194,6 +198,7 @@ __device__ __forceinline__ Segment prefix_segment(const PagedArgs& a, bool here)
   s.units = (s.n + a.unit_tok - 1) / a.unit_tok;
   s.pre = 0;
   s.causal = false;
+  s.cost = a.unit_cost;
   s.work = work_before(a, s, s.units);
   return s;
 }
@@ -209,6 +214,80 @@ struct ShareSmem {
   Segment seg;  // where the share begins: segment, request (-1: the prefix) and
   int b, off;   // unit within the segment
 };
+
+// Where both kernels of a call run at once, the wide one takes as many SMs as let
+// both end together, the narrow one the others. Here: the wide kernel's share per SM
+// of `units` row units with `work` units of work each, and what a row unit counts
+// then (a little more where it is cut in equal parts). us of an SM per unit of work:
+// the wide kernel's 2.5 for two tiles of a prefix or 1.7 for one, the narrow one's
+// 0.85 for two CTAs; the narrow kernel as a whole is not faster than HBM, 1.25 us per
+// unit and SM; the wide kernel spends 6 us more at its start and end (one B200,
+// D = 128; other head dimensions scale all).
+struct WideShare {
+  int per, work;
+};
+__host__ __device__ inline WideShare wide_share(const PagedArgs& a, int units, int work,
+                                                float narrow) {
+  const float total = (float)units * (float)work;
+  const float wide = total * (a.total_q * a.group <= kBM ? 1.7f : 2.5f);
+  // n (t - 6) = wide and (sms - n) t = own, the time t not below HBM's
+  const float sms = (float)a.ctas[0], own = 0.85f * narrow, b = 6.0f * sms + wide + own;
+  const float t = fmaxf((b + sqrtf(b * b - 24.0f * sms * own)) / (2.0f * sms), 1.25f * narrow / sms);
+  const float n = fmaxf(fminf(ceilf(wide / fmaxf(t - 6.0f, 1.0f)), sms - 1.0f), 1.0f);
+  const int per = (int)fmaxf(ceilf(total / n), 1.0f);
+  // whole row units, or equal parts of one, where that is near: a CTA with parts of
+  // two spends the start and the end of a row unit twice
+  if (per >= work) {
+    const int whole = per / work * work;
+    if (total <= (sms - 1.0f) * (float)whole && 4 * (per - whole) <= whole) return {whole, work};
+  } else {
+    const int parts = (work + per - 1) / per, part = (work + parts - 1) / parts;
+    if ((float)units * (float)parts <= sms - 1.0f) return {part, part * parts};
+  }
+  return {per, work};
+}
+
+// CTAs of the narrow kernel beside the wide one with that share.
+__host__ __device__ inline int ctas_beside(const PagedArgs& a, int units, const WideShare& w) {
+  const int left = a.ctas[0] - (int)ceilf((float)units * (float)w.work / (float)w.per);
+  return left < 1 ? 2 : 2 * left;
+}
+
+// This kernel's share per CTA, of `total` units. Beside the other kernel the wide
+// one has a prefix only, of which the row units may get longer.
+template <int THREADS>
+__device__ __forceinline__ int share_per_cta(const PagedArgs& a, ShareSmem<THREADS>& sm,
+                                             long long& total, Segment& prefix) {
+  int ctas = gridDim.x;
+  if (a.beside && a.requests_here) {
+    const int tokens = max(clamp_token(a, a.batch) - clamp_token(a, 0), 1);
+    const int units = (tokens + a.other_tok - 1) / a.other_tok * a.kv_heads;
+    const int work = (a.prefix_len + kBN - 1) / kBN + a.other_cost;
+    ctas = min(ctas, ctas_beside(a, units, wide_share(a, units, work, (float)total)));
+  } else if (a.beside) {
+    float narrow = 0.0f;
+#pragma unroll 1
+    for (int b = threadIdx.x; b < a.batch; b += THREADS)
+      narrow += (float)((own_tokens(a, b) + a.other_tok - 1) / a.other_tok) *
+                (float)(max(a.kv_lens[b], 0) / kBN + 1 + a.other_cost);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) narrow += __shfl_xor_sync(0xffffffffu, narrow, o);
+    if ((threadIdx.x & 31) == 0) sm.sum[threadIdx.x >> 5] = (long long)narrow;
+    __syncthreads();
+    long long sum = 0;
+#pragma unroll 1
+    for (int w = 0; w < THREADS / 32; ++w) sum += sm.sum[w];
+    if (prefix.units > 0) {
+      const int work = prefix.work / prefix.units;
+      const WideShare w = wide_share(a, prefix.units * a.kv_heads, work, (float)a.kv_heads * (float)sum);
+      prefix.cost += w.work - work;
+      prefix.work = prefix.units * w.work;
+      total = (long long)prefix.work * a.kv_heads;
+      return w.per;
+    }
+  }
+  return max((int)((total + ctas - 1) / ctas), 1);
+}
 
 // Every thread sums the work of a run of requests; a block scan gives the total,
 // and the thread that holds the CTA's first unit notes its segment. Called by
@@ -231,8 +310,8 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
     fat = !__syncthreads_or(thin);
   }
   Share r{0, 0, 1, fat ? (a.prefix_len + kBN - 1) / kBN : 0};
-  const Segment pre = prefix_segment(a, a.prefix_here && !fat);
-  const int pre_work = (int)min((long long)pre.work * a.kv_heads, (long long)kMostWork);
+  Segment pre = prefix_segment(a, a.prefix_here && !fat);
+  int pre_work = (int)min((long long)pre.work * a.kv_heads, (long long)kMostWork);
   long long mine = 0, base = 0, total = pre_work;
   // Two passes over the requests: their work, then (the thread that holds it) the
   // CTA's first unit.
@@ -273,9 +352,10 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
       if (threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
       break;
     }
-    r.per = max(1, ((int)total + (int)gridDim.x - 1) / (int)gridDim.x);
-    r.lo = min((int)blockIdx.x * r.per, (int)total);
-    r.hi = min(r.lo + r.per, (int)total);
+    r.per = share_per_cta(a, sm, total, pre);
+    pre_work = max(pre_work, pre.work * a.kv_heads);
+    r.lo = (int)min((long long)blockIdx.x * r.per, total);
+    r.hi = (int)min((long long)r.lo + r.per, total);
     if (r.lo < pre_work) {
       if (threadIdx.x == 0) {
         sm.b = -1;
@@ -321,6 +401,7 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
   Segment s;
   s.work = 0;
   s.units = 0;
+  s.cost = 0;
   // The lengths of the following segments are read again, one at a time. Lengths
   // that another stream changes meanwhile (a caller's mistake) must not lead out
   // of the tables: a position that is none ends the work.
@@ -341,9 +422,9 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
       at -= before;
     }
   }
-  const int cost = a.unit_cost;
 #pragma unroll 1
   while (true) {
+    const int cost = s.cost;
     Item item;
     item.request = kEnd;
     item.blocks = 0;
@@ -413,13 +494,17 @@ struct TileLoader {
     return a.num_blocks;
   }
   __device__ __forceinline__ void load(const PagedArgs& a, int head, const CUtensorMap* map,
-                                       void* tile, uint64_t* bar, int j, int block) const {
+                                       void* tile, uint64_t* bar, int j, int block,
+                                       bool once = false) const {
     if (lane == 0) mbar_arrive_expect_tx(bar, kBN * D * 2);
     __syncwarp();
     const int in = (j * kBN + row) & ((1 << a.rows_log2) - 1);
-    if (lane < boxes)
-      tma_load_3d(static_cast<uint8_t*>(tile) + half * kBoxBytes + row * 128, map, bar, 64 * half,
-                  (head << a.rows_log2) + in, block);
+    if (lane < boxes) {
+      uint8_t* dst = static_cast<uint8_t*>(tile) + half * kBoxBytes + row * 128;
+      const int x = 64 * half, y = (head << a.rows_log2) + in;
+      if (once) tma_load_3d_once(dst, map, bar, x, y, block);
+      else tma_load_3d(dst, map, bar, x, y, block);
+    }
   }
 };
 

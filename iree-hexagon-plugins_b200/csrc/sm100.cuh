@@ -216,6 +216,18 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map,
       : "memory");
 }
 
+// The same for data that is read once: its L2 lines are the first to be replaced.
+__device__ __forceinline__ void tma_load_3d_once(void* dst, const CUtensorMap* map,
+                                                 uint64_t* bar, int x, int y, int z) {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_"
+      "tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
+
 // Asks the TMA unit to bring a 2-D box of `map` into L2 (no shared-memory
 // destination, no completion signal). x is the innermost coordinate. L2 is
 // the device's point of coherence, so a prefetch issued before

@@ -316,6 +316,37 @@ def test_attention_paged_graphs_on_one_workspace(cuda_pkg):
     assert cuda_pkg.device_status() == 0
 
 
+@pytest.mark.parametrize("B,D,prefix,top", [(40, 128, 4096, 300), (64, 64, 9001, 40),
+                                            (200, 128, 1500, 900)])
+def test_attention_paged_both_kernels_follow_inputs_in_a_graph(cuda_pkg, B, D, prefix, top):
+    """A prefix and the requests' own keys side by side: lengths and queries that the
+    launch just before has written, replay after replay."""
+    b = Batch([1] * B, [(i * 37) % top for i in range(B)], 32, 8, D, 16, prefix, seed=3)
+    full = b.kv_lens.clone()
+    step, q0 = torch.zeros_like(full), b.q.clone()
+    want = []
+    for i in range(4):
+        b.kv_lens.copy_((full - i * 16).clamp_(min=0))
+        b.lens = b.kv_lens.tolist()
+        b.q.copy_(q0.roll(i, 0))
+        torch.cuda.synchronize()
+        b.check(cuda_pkg, max_q_len=1)
+        want.append(b.run(cuda_pkg, max_q_len=1).clone())
+    out = torch.empty_like(want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.kv_lens.copy_(torch.clamp(full - step * 16, min=0))
+        b.q.copy_(torch.index_select(q0, 0, (torch.arange(B, device=DEV) - step[0]) % B))
+        b.run(cuda_pkg, max_q_len=1, out=out)
+    for i in (0, 3, 1, 2, 0, 1, 3):
+        step.fill_(i)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i])
+    assert cuda_pkg.device_status() == 0
+
+
 def test_attention_paged_bad_indices_are_reported_not_followed(cuda_pkg):
     b = Batch([1, 1], [40, 300], 8, 2, 128, 16, 100, seed=13)
     want = b.run(cuda_pkg).clone()
