@@ -6,7 +6,8 @@
 //   O^T[d, q] += V^T P^T   (M = 128 d, N = 16, K = 128 keys)
 // so that a block of 128 keys costs each thread one exponential per live row
 // and the tensor core next to nothing. Bound: HBM, one K and one V tile per
-// block; everything else has to hide behind the loads:
+// block, 1.3 us a block and SM where they stream from HBM and 0.85 from L2 (one
+// B200, D = 128, 4 rows); everything else has to hide behind the loads:
 //   * two CTAs per SM, each with a three-tile ring;
 //   * S of the next two blocks is computed ahead of the softmax (two TMEM
 //     buffers), across items too, and Q is double-buffered: short requests

@@ -10,7 +10,8 @@
 //     merges the two accumulators in the epilogue, so that short units do not
 //     wait for one softmax chain per block.
 // Bound: the tensor core and the exponentials, 2.0 us per 256 x 128 block at
-// D = 128 (1.1 PFLOP/s), where the keys are many. One CTA per SM, persistent.
+// D = 128 (1.1 PFLOP/s), where the keys are many; 2.6 us beside a narrow kernel
+// that saturates HBM. One CTA per SM, persistent.
 #pragma once
 
 #include "paged_work.cuh"

@@ -11,7 +11,8 @@
 // unit_cost more for its start and end) -- prefix, request 0, request 1 ...;
 // inside a segment KV head by KV head, row unit by row unit -- and CTA i takes
 // units [i S, (i + 1) S), S = ceil(T / CTAs): equal shares whatever the lengths,
-// which are read on the GPU. The part of a row unit's blocks that falls to one CTA is an item;
+// which are read on the GPU (where both kernels run at once, of the CTAs that each
+// has then). The part of a row unit's blocks that falls to one CTA is an item;
 // a row unit cut between CTAs leaves one partial result per CTA.
 #pragma once
 
