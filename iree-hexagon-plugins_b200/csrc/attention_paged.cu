@@ -254,8 +254,24 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     w.beside = narrow;
     w.other_tok = nr / a.group;
     w.other_cost = kNarrowUnitCost;
-    s = launch_pdl(attention_paged_wide_kernel<D>, dim3((unsigned)dev.num_sms), dim3(kThreads),
-                   WideSmem<D>::kAlloc, stream, "paged attention launch", tmQ, tmK, tmV, w);
+    // Beside the narrow kernel in clusters of two CTAs, which share a TPC: the CTAs
+    // without work leave both SMs of one, and a wide CTA that has a narrow one's
+    // loads on the other SM of its TPC takes a third longer.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)dev.num_sms);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = WideSmem<D>::kAlloc;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = narrow && dev.num_sms % 2 == 0 ? 2 : 1;
+    s = cuda_status(cudaLaunchKernelEx(&cfg, attention_paged_wide_kernel<D>, tmQ, tmK, tmV, w),
+                    "paged attention launch");
     if (s != HXB_OK) return s;
   }
   if (narrow) {
