@@ -16,7 +16,7 @@
 // one (attention_paged_wide.cuh, rows on the lanes, bound by the tensor core)
 // those of other batches and a prefix that many rows share. A decode batch behind
 // a long prefix has both at once, each on its share of the SMs (256 requests of
-// 550 keys behind 4096: 119 us, one kernel after the other 153). A combine kernel
+// 550 keys behind 4096: 115 us, one kernel after the other 153). A combine kernel
 // merges what each row has. K and V blocks come through 3-D tensor maps, one TMA
 // box per cache block and 64 columns, straight into the 128B-swizzled tile.
 //

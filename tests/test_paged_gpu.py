@@ -293,6 +293,24 @@ def test_attention_paged_two_streams(cuda_pkg):
         assert all(torch.equal(x, w) for x in g)
 
 
+def test_attention_paged_two_streams_with_both_kernels(cuda_pkg):
+    """The same where each call has its two kernels side by side, beside other work."""
+    batches = [Batch([1] * 60, [30 + i * s for i in range(60)], 32, 8, 128, 16, p, seed=s)
+               for s, p in ((11, 4000), (12, 9000))] + [Batch([150, 90], [300, 90], 32, 8, 128, 16, 400)]
+    want = [b.run(cuda_pkg, max_q_len=max(b.new)).clone() for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = [[] for _ in batches]
+    for _ in range(8):
+        for i, (b, s) in enumerate(zip(batches, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(b.run(cuda_pkg, max_q_len=max(b.new)))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
+    assert cuda_pkg.device_status() == 0
+
+
 def test_attention_paged_graphs_on_one_workspace(cuda_pkg):
     """Graphs of both kernels and eager calls take turns on one workspace."""
     batches = [Batch([1] * 20, [30 + i * s for i in range(20)], 32, 8, 128, 16, p, seed=s)
