@@ -235,7 +235,9 @@ __host__ __device__ inline WideShare wide_share(const PagedArgs& a, int units, i
   const float sms = (float)a.ctas[0], own = 0.85f * narrow, b = 6.0f * sms + wide + own;
   const float t = fmaxf((b + sqrtf(b * b - 24.0f * sms * own)) / (2.0f * sms), 1.25f * narrow / sms);
   const float n = fmaxf(fminf(ceilf(wide / fmaxf(t - 6.0f, 1.0f)), sms - 1.0f), 1.0f);
-  const int per = (int)fmaxf(ceilf(total / n), 1.0f);
+  // (a call of more than kMostWork is not run, but its shares are computed, on the
+  // host too: an int all the same)
+  const int per = (int)fminf(fmaxf(ceilf(total / n), 1.0f), (float)kMostWork);
   // whole row units, or equal parts of one, where that is near: a CTA with parts of
   // two spends the start and the end of a row unit twice
   if (per >= work) {

@@ -387,6 +387,23 @@ def test_attention_paged_bad_indices_are_reported_not_followed(cuda_pkg):
     assert cuda_pkg.device_status() == 0
 
 
+@pytest.mark.parametrize("keys", [1 << 30, 33 << 20])
+def test_attention_paged_call_beyond_the_work_limit_is_reported(cuda_pkg, keys):
+    """A prefix of one block over and over, for so many rows that the call is above
+    2^30 pairs of a query tile and a key block: it returns and says so."""
+    n, Hq, Hkv, P, D = 2048, 1024, 64, 1024, 64
+    keys = min(keys, (1 << 30) - 1)
+    k = torch.zeros(1, Hkv, P, D, dtype=torch.float16, device=DEV)
+    q = torch.zeros(n, Hq, D, dtype=torch.float16, device=DEV)
+    table = torch.zeros(1, (1 << 20) - 1, **I32)
+    assert cuda_pkg.device_status() == 0
+    cuda_pkg.attention_paged(q, k, k, torch.tensor([0, n], **I32), torch.tensor([2100], **I32), table,
+                             prefix_table=torch.zeros(1 << 20, **I32), prefix_len=keys, max_q_len=1)
+    torch.cuda.synchronize()
+    assert cuda_pkg.device_status() == 2
+    Batch([1] * 20, [30 + i for i in range(20)], 32, 8, 128, 16, 900).check(cuda_pkg, max_q_len=1)
+
+
 # --------------------------------------------------------------------- tables
 def plain_tables(cached, new, free, cursor, table, P, max_tokens):
     """The definition, request by request."""
