@@ -217,12 +217,13 @@ __global__ void __launch_bounds__(kNarThreads, 2)
   const Share share = find_share(args, share_smem);
 
   // A reader's position in the items (each in shared memory until every reader
-  // has released it).
+  // has released it). A reader that runs ahead of the key threads (the Q warp passes
+  // over items without keys) waits here until their item, which may be long, has ended.
   Ring<kNarItems> it;
   auto get = [&](uint32_t n) -> const Item* {
     Ring<kNarItems> at;
     at.n = n;
-    const bool ok = wait_bar(&item_full[at.slot()], at.parity(), fs);
+    const bool ok = wait_bar(&item_full[at.slot()], at.parity(), fs, kLongWaitNs);
     return __all_sync(0xffffffffu, ok) ? &items[at.slot()] : nullptr;
   };
   auto release = [&]() {
@@ -387,7 +388,9 @@ __global__ void __launch_bounds__(kNarThreads, 2)
                                                    idx % kChunks * 8);
           }
         }
-        if (!__all_sync(0xffffffffu, wait_bar(&q_empty[q_ring.slot()], q_ring.parity() ^ 1, fs)))
+        // (the buffer's last unit may still be at work, for as long as it takes)
+        if (!__all_sync(0xffffffffu, wait_bar(&q_empty[q_ring.slot()], q_ring.parity() ^ 1, fs,
+                                              kLongWaitNs)))
           break;
         uint8_t* dst = smem + L::kOffQ + q_ring.slot() * L::kQBytes;
 #pragma unroll

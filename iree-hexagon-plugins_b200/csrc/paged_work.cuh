@@ -351,7 +351,7 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
         total += sm.sum[w];
       }
     }
-    if (total >= kMostWork) {  // (hours of work: not started)
+    if (total >= kMostWork) {  // (many seconds of work: not started)
       if (threadIdx.x == 0) atomicOr(a.status, kStatusBadIndex);
       break;
     }
@@ -373,21 +373,23 @@ __device__ __forceinline__ Share find_share(const PagedArgs& a, ShareSmem<THREAD
   return r;
 }
 
-// mbar_wait with its loop out of line: the roles of these kernels wait in many
-// places, and what runs once per item should not be fetched anew for each.
-static __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
-                                              int* status) {
-  return mbar_wait(bar, parity, FailState{abort, status});
-}
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const FailState& fs) {
-  if (mbar_try_wait(bar, parity)) return true;
-  return wait_slow(bar, parity, fs.abort, fs.status);
-}
-
 // Limit of a wait that a correct call may spend a large part of its time in (for a
 // tile to zero, for a long item's end): a launch that is stuck ends by the limit of
-// another role's wait, whose flag these waits watch.
+// another role's wait, whose flag these waits watch. The most work of a call
+// (kMostWork for each kernel) takes less than a minute.
 constexpr unsigned long long kLongWaitNs = 32 * kWaitLimitNs;
+
+// mbar_wait_for with its loop out of line: the roles of these kernels wait in many
+// places, and what runs once per item should not be fetched anew for each.
+static __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                              int* status, unsigned long long limit_ns) {
+  return mbar_wait_for(bar, parity, FailState{abort, status}, limit_ns);
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, const FailState& fs,
+                                         unsigned long long limit_ns = kWaitLimitNs) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return wait_slow(bar, parity, fs.abort, fs.status, limit_ns);
+}
 
 // Publishes the CTA's items, one after the other, into a ring of N records (one
 // thread). item_empty[] collects one arrival of every reader of a record.
@@ -463,7 +465,7 @@ __device__ __forceinline__ void announce(const PagedArgs& a, const Share& sh,
     }
     uint64_t* free_slot = &item_empty[out.slot()];
     const uint32_t parity = out.parity() ^ 1;
-    if (!(OUT_OF_LINE ? wait_bar(free_slot, parity, fs)
+    if (!(OUT_OF_LINE ? wait_bar(free_slot, parity, fs, kLongWaitNs)
                       : mbar_wait_for(free_slot, parity, fs, kLongWaitNs)))
       return;
     items[out.slot()] = item;

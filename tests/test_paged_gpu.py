@@ -276,6 +276,48 @@ def test_attention_paged_call_of_seconds(cuda_pkg):
     assert bool(((got[some].double() - want).abs() <= bound).all())
 
 
+def counting_caches(ids, Hkv, P, D):
+    """K of zeros (every visible key has the same weight) and V that says where a row
+    comes from: block i of head h has a one in column (8 i + row // 128 + h) % D."""
+    k = torch.zeros(ids, Hkv, P, D, dtype=torch.float16, device=DEV)
+    i, h, r = (torch.arange(n, device=DEV) for n in (ids, Hkv, P))
+    col = (8 * i[:, None, None] + r[None, None] // 128 + h[None, :, None]) % D
+    return k, torch.nn.functional.one_hot(col, D).half()
+
+
+def counted(times, Hkv, D):
+    """[Hkv, D] outputs for a table with times[i] entries of block i (of 1024 rows)."""
+    want = torch.zeros(Hkv, D, dtype=torch.float64)
+    for i, n in enumerate(times):
+        for g in range(8):
+            for h in range(Hkv):
+                want[h, (8 * i + g + h) % D] += n
+    return (want / (8 * sum(times))).to(DEV)
+
+
+@pytest.mark.parametrize("short", [0, 5])
+def test_attention_paged_long_item_of_the_narrow_kernel(cuda_pkg, short):
+    """A decode request whose part of one CTA lasts longer than the limit of one wait
+    (2.8 million key blocks), and 100 short items (one per KV head, with and without
+    keys) behind it in the same CTA. Sums of weights and of V are whole numbers below
+    2^24 or rounded by 2^-24, the log2 of a piece's sum (below 32) by 1.5 * 2^-19, so the
+    f16 result is off by 2^-11 + 2^-17 of its value at most."""
+    Hkv, P, D, cols = 100, 1024, 128, (1 << 20) - 1
+    times = [300001, cols - 300001]
+    k, v = counting_caches(2, Hkv, P, D)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    table = torch.zeros(2, cols, **I32)
+    table[0, torch.randperm(cols, device=DEV, generator=g)[:times[1]]] = 1
+    q = torch.randn(2, Hkv, D, device=DEV, generator=g).half()
+    got = cuda_pkg.attention_paged(q, k, v, torch.tensor([0, 1, 2], **I32),
+                                   torch.tensor([cols * P, short], **I32), table, max_q_len=1).double()
+    torch.cuda.synchronize()
+    assert cuda_pkg.device_status() == 0
+    want = counted(times, Hkv, D)
+    assert bool(((got[0] - want).abs() <= (2 ** -11 + 2 ** -17) * want).all())
+    assert torch.equal(got[1], v[0, :, 0].double() * (short > 0))
+
+
 def test_attention_paged_two_streams(cuda_pkg):
     """Calls with workspaces of their own may run at the same time."""
     batches = [Batch([1] * 20, [30 + i * s for i in range(20)], 32, 8, 128, 16, 900, seed=s)
