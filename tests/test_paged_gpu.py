@@ -295,6 +295,28 @@ def counted(times, Hkv, D):
     return (want / (8 * sum(times))).to(DEV)
 
 
+def test_attention_paged_call_of_seconds_counts_every_block(cuda_pkg):
+    """A call of the wide kernel of some seconds: 16 cache blocks in a shuffled table, each
+    so often as no other. A key block lost or taken twice changes a column by 1 / 900 of
+    its value or more, above twice the bound. Weights and V are ones, their sums whole
+    numbers below 2^24; what is rounded is the quotient (2^-22), the log2 of a cut unit's
+    sum (below 32, 1.5 * 2^-19) and the f16 result, by 2^-11 + 2^-17 of its value at
+    most."""
+    n, Hq, Hkv, P, D = 16384, 32, 8, 1024, 128
+    times = list(range(600, 920, 20))
+    k, v = counting_caches(16, Hkv, P, D)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    table = torch.arange(16, **I32).repeat_interleave(torch.tensor(times, device=DEV))
+    table = table[torch.randperm(sum(times), device=DEV, generator=g)][None]
+    q = torch.randn(n, Hq, D, device=DEV, generator=g).half()
+    got = cuda_pkg.attention_paged(q, k, v, torch.tensor([0, n], **I32),
+                                   torch.tensor([P * sum(times)], **I32), table, causal=False)
+    torch.cuda.synchronize()
+    assert cuda_pkg.device_status() == 0
+    want = counted(times, Hkv, D).repeat_interleave(Hq // Hkv, 0)
+    assert bool(((got.double() - want).abs() <= (2 ** -11 + 2 ** -17) * want).all())
+
+
 @pytest.mark.parametrize("short", [0, 5])
 def test_attention_paged_long_item_of_the_narrow_kernel(cuda_pkg, short):
     """A decode request whose part of one CTA lasts longer than the limit of one wait
