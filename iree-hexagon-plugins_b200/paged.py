@@ -91,7 +91,8 @@ def paged_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks:
     -1 behind the last token, cursor_out [2]: the next cursor and how many
     blocks were missing). Outputs may be given: `kv_lens` may be `cached_lens`
     and `cursor_out` may be `cursor` (of 2 elements). `max_tokens` is needed
-    unless `slots` is given, whose length it then is."""
+    unless `slots` is given, whose length it then is; of a longer `slots` its
+    first max_tokens entries are written and returned."""
     lib = _native.load()
     index = cached_lens.get_device()
     if index < 0 or block_rows < 1:
@@ -120,7 +121,8 @@ def paged_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, free_blocks:
             _ints("q_start", q_start, _I32, B + 1, index), _ints("kv_lens", kv_lens, _I32, B, index),
             _ints("slots", slots, _I64, n, index), n,
             _ints("cursor_out", cursor_out, _I32, 2, index)), _raw_stream(index)))
-    return q_start, kv_lens, slots, cursor_out
+    # (what lies behind them is an earlier step's: not for this step's cache write)
+    return q_start, kv_lens, slots if slots.numel() == n else slots.view(-1)[:n], cursor_out
 
 
 def kv_cache_write_paged(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torch.Tensor,

@@ -545,6 +545,26 @@ def test_paged_tables_in_place(cuda_pkg, B, new_max):
     assert cuda_pkg.device_status() == 0
 
 
+def test_paged_tables_returns_the_slots_of_its_step_only(cuda_pkg):
+    """A slot buffer kept from a longer step: the entries behind max_tokens are the old
+    step's, and rows of the cache write must not reach them."""
+    def step(new, **kw):
+        return cuda_pkg.paged_tables(torch.zeros(1, **I32), torch.tensor([new], **I32),
+                                     torch.arange(10, **I32), torch.zeros(1, **I32),
+                                     torch.zeros(1, 4, **I32), block_rows=16, **kw)[2]
+    buf = step(20, max_tokens=24)
+    assert buf.tolist() == list(range(20)) + [-1] * 4
+    got = step(3, max_tokens=5, slots=buf)
+    assert got.tolist() == [0, 1, 2, -1, -1] and got.data_ptr() == buf.data_ptr()
+    assert step(3, slots=buf) is buf and buf.tolist() == [0, 1, 2] + [-1] * 21
+    assert step(2, max_tokens=3, slots=buf.view(4, 6)).tolist() == [0, 1, -1]
+    k = torch.zeros(4, 1, 16, 64, dtype=torch.float16, device=DEV)
+    rows = torch.ones(20, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(ValueError, match="slots"):  # more rows than the step has tokens
+        cuda_pkg.kv_cache_write_paged(rows, rows, k, k.clone(), got)
+    assert cuda_pkg.device_status() == 0
+
+
 def test_paged_tables_out_of_range_is_reported(cuda_pkg):
     def call(cached, new, cursor=0, n=8, cols=4):
         t = torch.zeros(len(cached), cols, **I32)
