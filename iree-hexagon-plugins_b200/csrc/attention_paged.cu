@@ -431,6 +431,7 @@ extern "C" hxb_status_t hxb_attention_paged_f16(const hxb_attention_paged_t* arg
   }
   a.status = dev->status_word;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return head_dim == 64 ? launch_paged<64>(tmQ, tmK, tmV, a, max_q_len, *dev, st)
-                        : launch_paged<128>(tmQ, tmK, tmV, a, max_q_len, *dev, st);
+  const int64_t most = std::min(max_q_len, total_q);  // (no request has more tokens)
+  return head_dim == 64 ? launch_paged<64>(tmQ, tmK, tmV, a, most, *dev, st)
+                        : launch_paged<128>(tmQ, tmK, tmV, a, most, *dev, st);
 }

@@ -174,6 +174,17 @@ def test_attention_paged_max_q_len_is_a_hint(cuda_pkg, hint):
     Batch([1, 30, 2, 1], [50, 30, 129, 1], 8, 2, 128, 16, 140, seed=3).check(cuda_pkg, max_q_len=hint)
 
 
+@pytest.mark.parametrize("new", [[1, 2], [1, 30, 2, 1]])
+def test_attention_paged_hints_above_the_batch_are_all_its_tokens(cuda_pkg, new):
+    """A hint of more tokens than the batch has, the largest number among them, is the
+    same as all its tokens: the same kernels, so the same bits."""
+    b = Batch(new, [50 + 9 * i for i in range(len(new))], 8, 2, 128, 16, 140, seed=3)
+    want = b.run(cuda_pkg, max_q_len=sum(new)).clone()
+    for hint in (sum(new) + 5, 2 ** 61, 2 ** 63 - 1):
+        b.check(cuda_pkg, max_q_len=hint)
+        assert torch.equal(b.run(cuda_pkg, max_q_len=hint), want)
+
+
 def test_attention_paged_padded_rows_and_block_stride(cuda_pkg):
     """Rows around the batch's are left as they are; K and V blocks may be
     further apart than they are long."""
