@@ -32,7 +32,12 @@ _WRITE = struct.Struct("=QQqQqQQqqqqq")
 _ATTENTION = struct.Struct("=QqQqQQqqqQQqqqQqqQqqqqfiQQ")
 _NO_GUARD = contextlib.nullcontext()
 _I32, _I64, _F16 = torch.int32, torch.int64, torch.float16
-_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _raw_stream(index: int) -> int:
+    """Handle of the device's current stream (torch.cuda.current_stream makes an
+    object first: 1.3 us instead of 0.1, of a call of 6 to 13)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _on(device: torch.device):

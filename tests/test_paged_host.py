@@ -3,8 +3,12 @@ before any device access (no GPU needed; the pointers are never followed)."""
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 
 import pytest
+
+from conftest import REPO
 
 A = 0x100000  # an aligned address
 
@@ -147,3 +151,14 @@ def test_python_entries_refuse_before_the_library(pkg):
     ints = torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
         pkg.paged_tables(ints, ints, ints, ints, ints[None], block_rows=16, max_tokens=1)
+
+
+def test_package_imports_on_a_torch_without_cuda_bindings():
+    """The streams of a call are looked up by the call, not by the import."""
+    program = ("import torch\n"
+               "for name in [n for n in vars(torch._C) if n.startswith('_cuda_')]:\n"
+               "    delattr(torch._C, name)\n"
+               "import __graft_entry__\n"
+               "assert callable(__graft_entry__.load_package().attention_paged)\n")
+    r = subprocess.run([sys.executable, "-c", program], cwd=REPO, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
