@@ -56,6 +56,11 @@ def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, numel: int, index: int
     return t.data_ptr()
 
 
+def _pitches(t: torch.Tensor) -> tuple[int, ...]:
+    """Strides of `t`, 0 for an axis of one element, where any is as good."""
+    return tuple(s if n > 1 else 0 for n, s in zip(t.shape, t.stride()))
+
+
 def _table(t: torch.Tensor, rows: int, index: int) -> tuple[int, int, int]:
     """(pointer, row pitch, columns) of a block table."""
     if t.dim() != 2 or t.dtype is not _I32 or t.get_device() != index or t.shape[0] != rows or \
@@ -75,7 +80,10 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int,
         raise ValueError("k_cache / v_cache must be f16 [blocks, kv_heads, block_rows, head_dim]")
     n, h, p, d = shape
     stride = k_cache.stride()
-    if v_cache.stride() != stride or stride[1:] != (p * d, d, 1):
+    if (v_cache.stride() != stride or stride[1:] != (p * d, d, 1)) and \
+            (_pitches(v_cache) != _pitches(k_cache) or
+             _pitches(k_cache)[1:] != tuple(s if m > 1 else 0 for m, s in
+                                            ((h, p * d), (p, d), (d, 1)))):
         raise ValueError("the blocks of k_cache / v_cache must be contiguous, with one stride")
     index = k_cache.get_device()
     if index < 0 or v_cache.get_device() != index:
@@ -141,7 +149,8 @@ def kv_cache_write_paged(k_src: torch.Tensor, v_src: torch.Tensor, k_cache: torc
     index, blocks, heads, rows, D, stride = _cache(k_cache, v_cache)
     shape, src_stride = k_src.shape, k_src.stride()
     if len(shape) != 2 or shape[1] != heads * D or shape != v_src.shape or src_stride[1] != 1 or \
-            src_stride != v_src.stride() or k_src.dtype is not _F16 or v_src.dtype is not _F16:
+            (src_stride != v_src.stride() and _pitches(k_src) != _pitches(v_src)) or \
+            k_src.dtype is not _F16 or v_src.dtype is not _F16:
         raise ValueError("k_src / v_src must be f16 [tokens, kv_heads * head_dim] views of one layout "
                          "with unit inner stride")
     if k_src.get_device() != index or v_src.get_device() != index:
@@ -186,7 +195,8 @@ def attention_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     lib = _native.load()
     index, blocks, Hkv, rows, D, stride = _cache(k_cache, v_cache)
     shape, q_stride = query.shape, query.stride()
-    if len(shape) != 3 or shape[2] != D or q_stride[2] != 1 or q_stride[1] != D or \
+    if len(shape) != 3 or shape[2] != D or q_stride[2] != 1 or \
+            (q_stride[1] != D and shape[1] > 1) or \
             query.dtype is not _F16 or query.get_device() != index:
         raise ValueError("query must be f16 [tokens, q_heads, head_dim] with contiguous heads on the "
                          "caches' device")
@@ -196,7 +206,7 @@ def attention_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         o_stride = out.stride()
     else:
         o_stride = out.stride()
-        if out.shape != shape or o_stride[2] != 1 or o_stride[1] != D or \
+        if out.shape != shape or o_stride[2] != 1 or (o_stride[1] != D and shape[1] > 1) or \
                 out.dtype is not _F16 or out.get_device() != index:
             raise ValueError("out must match query's shape, type and device, with contiguous heads")
     if n == 0:

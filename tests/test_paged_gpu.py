@@ -192,6 +192,31 @@ def test_attention_paged_padded_rows_and_block_stride(cuda_pkg):
     Batch([1, 1], [20, 300], 4, 2, 64, 32, 0, pad=(1, 2), spread=1).check(cuda_pkg, max_q_len=1)
 
 
+def test_paged_entries_take_any_stride_of_an_axis_of_one(cuda_pkg):
+    """One head: [blocks, rows, 1, D] storage is [blocks, 1, rows, D] too, and a query
+    may be columns of wider rows. One token: its pitch is no matter."""
+    g = torch.Generator(device=DEV).manual_seed(7)
+    P, D, n = 16, 64, 5
+    src = torch.randn(n, 4 * D, device=DEV, generator=g).half()
+    slots = torch.arange(n, device=DEV) + 3
+    seen = []
+    for odd in (False, True):
+        k, v = (torch.zeros(2, P, D, dtype=torch.float16, device=DEV)
+                .as_strided((2, 1, P, D), (P * D, D if odd else P * D, D, 1)) for _ in "kv")
+        q = src.as_strided((n, 1, D), (4 * D, 4 * D if odd else D, 1))
+        out = torch.zeros(n, 4 * D, dtype=torch.float16, device=DEV).as_strided(q.shape, q.stride())
+        cuda_pkg.kv_cache_write_paged(src[1:, D:2 * D], src[1:, 2 * D:3 * D], k, v, slots[1:])
+        k0, v0 = src[:1, D:2 * D], src[:1, 2 * D:3 * D]
+        cuda_pkg.kv_cache_write_paged(k0, v0.clone() if odd else v0, k, v, slots)
+        cuda_pkg.attention_paged(q, k, v, torch.tensor([0, n], **I32), torch.tensor([n + 3], **I32),
+                                 torch.zeros(1, 1, **I32), out=out)
+        seen.append((k, v, out))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(*seen))
+    assert torch.equal(seen[1][0][0, 0, 3:8], src[:, D:2 * D]) and bool((seen[1][2] != 0).any())
+    assert cuda_pkg.device_status() == 0
+
+
 @pytest.mark.parametrize("junk", [float("inf"), -65504.0, 65504.0])
 def test_attention_paged_ignores_rows_behind_the_lengths(cuda_pkg, junk):
     Batch([1, 4], [130, 7], 8, 2, 128, 64, 33, junk=junk).check(cuda_pkg)
