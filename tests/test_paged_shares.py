@@ -1,9 +1,11 @@
 """How a paged attention call is cut between its two kernels (paged_work.cuh),
 compiled for the host and swept over sizes up to the entry's limits (no GPU
 needed): the shares are positive numbers and the grids fit the workspace, also for
-the calls that are too large to run."""
+the calls that are too large to run. And the order of the launch dependencies that
+lets the two run at once, read from the source."""
 from __future__ import annotations
 
+import re
 import subprocess
 
 import pytest
@@ -59,3 +61,34 @@ def test_shares_of_the_two_kernels_are_numbers_at_every_size(tmp_path):
     assert r.returncode == 0, r.stderr[-2000:]
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, f"status {r.returncode}: {r.stdout}"
+
+
+def kernel_body(name):
+    """The kernel's source behind its signature, without comments."""
+    text = (CSRC / f"attention_paged_{name}.cuh").read_text()
+    body = text[text.index(f"attention_paged_{name}_kernel("):]
+    return re.sub(r"//.*", "", body)
+
+
+def test_the_narrow_kernel_starts_when_all_before_the_wide_one_has_ended():
+    """Beside the wide kernel the narrow one reads the inputs without a wait: it starts
+    when every CTA of the wide one has triggered, which each does behind its own wait
+    for all that came before. No path may trigger, or end, ahead of that wait."""
+    wide = kernel_body("wide")
+    assert wide.count("pdl_wait();") == wide.count("pdl_trigger();") == 1
+    before, after = wide.split("pdl_wait();")
+    assert "return" not in before and "pdl_trigger" not in before
+    assert re.match(r"\s*pdl_trigger\(\);", after)  # at the top level, for all threads
+    assert before.count("{") - before.count("}") == 1
+
+
+def test_the_narrow_kernel_ends_behind_the_wide_one():
+    """The combine kernel waits for the narrow one only, so no path of that one may let
+    it start early or end without having waited for the wide one."""
+    narrow = kernel_body("narrow")
+    assert "pdl_trigger" not in narrow
+    first, second, rest = narrow.split("pdl_wait();")
+    assert re.search(r"if \(args\.beside\) \{[^{}]*\} else \{\s*$", first)
+    assert re.search(r"if \(args\.beside\) $", second) and re.match(r"\s*\}\s*\}", rest)
+    roles = second[second.index("if (warp == 0) {"):]
+    assert not re.search(r"^  return", roles, re.M)  # (returns of the roles' lambdas only)
