@@ -581,6 +581,21 @@ def test_paged_tables_in_place(cuda_pkg, B, new_max):
     assert cuda_pkg.device_status() == 0
 
 
+def test_paged_tables_in_place_at_the_largest_batch(cuda_pkg):
+    """Lengths and cursor over themselves for 16384 requests (a cluster whose CTAs fill
+    their shared memory), the free list short of a few blocks."""
+    cached, new, free, table, n = tables_case(16384, 3, 40, 8, 5, short=12)
+    lens, cur, t = torch.tensor(cached, **I32), torch.tensor([2, 0], **I32), torch.tensor(table, **I32)
+    q_start, kv_lens, slots, cursor = cuda_pkg.paged_tables(
+        lens, torch.tensor(new, **I32), torch.tensor(free, **I32), cur, t, block_rows=8,
+        max_tokens=n, kv_lens=lens, cursor_out=cur)
+    want = plain_tables(cached, new, free, 2, table, 8, n)
+    assert want[3][1] > 0
+    got = [x.tolist() for x in (q_start, kv_lens, slots, cursor)]
+    assert got == list(want) and t.tolist() == table
+    assert cuda_pkg.device_status() == 0
+
+
 def test_paged_tables_returns_the_slots_of_its_step_only(cuda_pkg):
     """A slot buffer kept from a longer step: the entries behind max_tokens are the old
     step's, and rows of the cache write must not reach them."""
