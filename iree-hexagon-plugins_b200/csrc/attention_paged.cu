@@ -16,9 +16,10 @@
 // one (attention_paged_wide.cuh, rows on the lanes, bound by the tensor core)
 // those of other batches and a prefix that many rows share. A decode batch behind
 // a long prefix has both at once, each on its share of the SMs (256 requests of
-// 550 keys behind 4096: 115 us, one kernel after the other 153). A combine kernel
-// merges what each row has. K and V blocks come through 3-D tensor maps, one TMA
-// box per cache block and 64 columns, straight into the 128B-swizzled tile.
+// 550 keys behind 4096: 115 us, one kernel after the other in the same code 143). A
+// combine kernel merges what each row has. K and V blocks come through 3-D tensor
+// maps, one TMA box per cache block and 64 columns, straight into the 128B-swizzled
+// tile.
 //
 // The reference's KV-cache models attend one contiguous cache with one length
 // for the batch (integration_tests/models/kv_cache.py:46-112); the shared
@@ -40,6 +41,7 @@ namespace {
 // takes 2.05 us per 256 rows or 1.4 for the last 128; a second kernel costs the call
 // 3 us (one B200, D = 128, 8 KV heads: 64 rows on 16 blocks 23.0 us narrow, 25.9
 // wide; 128 rows on 32 blocks 47.1 us narrow, 35.8 wide, with the step's tables).
+// Both sides were measured at D = 128 only; D = 64 goes by the same numbers.
 bool prefix_to_narrow(int64_t rows, int64_t blocks, int64_t kv_heads, int num_sms) {
   const double narrow = (double)((rows + 15) / 16) * 0.85;
   const double wide = rows <= 128 ? 1.4 : (double)((rows + 255) / 256) * 2.05;
@@ -230,8 +232,9 @@ hxb_status_t launch_paged(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
   if (s != HXB_OK) return s;
   // Batches whose requests are expected to have at most 16 rows per KV head go to
   // the narrow kernel, others to the wide one (its solo mode is as near to HBM
-  // on a long request; a launch of the narrow kernel for the short requests of a
-  // mixed batch cost more than it saved).
+  // on a long request). So one longer request takes the whole batch there: a second
+  // launch for the short requests of a mixed batch cost more than it saved when the
+  // two kernels ran one after the other, and has not been measured beside the other.
   const int narrow_tok = kNarrowRows / a.group;
   const bool narrow = narrow_tok > 0 && max_q_len <= narrow_tok;
   const bool prefix = a.prefix_len > 0;

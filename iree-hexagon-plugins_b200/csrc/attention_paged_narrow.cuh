@@ -6,8 +6,9 @@
 //   O^T[d, q] += V^T P^T   (M = 128 d, N = 16, K = 128 keys)
 // so that a block of 128 keys costs each thread one exponential per live row
 // and the tensor core next to nothing. Bound: HBM, one K and one V tile per
-// block, 1.3 us a block and SM where they stream from HBM and 0.85 from L2 (one
-// B200, D = 128, 4 rows); everything else has to hide behind the loads:
+// block, 1.4 us a block and SM where they stream from HBM and 0.70 from L2 (one
+// B200, D = 128, 4 rows, 37 long requests of 8 KV heads; 16 rows 0.75 from L2; D = 64
+// 0.68 and 0.63); everything else has to hide behind the loads:
 //   * two CTAs per SM, each with a three-tile ring;
 //   * S of the next two blocks is computed ahead of the softmax (two TMEM
 //     buffers), across items too, and Q is double-buffered: short requests

@@ -9,9 +9,10 @@
 //     softmax warpgroups alternate key blocks of the SAME tile ("solo") and
 //     merges the two accumulators in the epilogue, so that short units do not
 //     wait for one softmax chain per block.
-// Bound: the tensor core and the exponentials, 2.0 us per 256 x 128 block at
-// D = 128 (1.1 PFLOP/s), where the keys are many; 2.6 us beside a narrow kernel
-// that saturates HBM. One CTA per SM, persistent.
+// Bound: the tensor core and the exponentials, 2.05 to 2.15 us per 256 x 128 block
+// at D = 128 (1.2 PFLOP/s), where the keys are many, 2.1 at D = 64 (the exponentials
+// are the same); 2.6 us (D = 128) beside a narrow kernel that saturates HBM. One CTA
+// per SM, persistent.
 #pragma once
 
 #include "paged_work.cuh"

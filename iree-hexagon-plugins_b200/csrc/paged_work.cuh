@@ -219,11 +219,13 @@ struct ShareSmem {
 // Where both kernels of a call run at once, the wide one takes as many SMs as let
 // both end together, the narrow one the others. Here: the wide kernel's share per SM
 // of `units` row units with `work` units of work each, and what a row unit counts
-// then (a little more where it is cut in equal parts). us of an SM per unit of work:
-// the wide kernel's 2.5 for two tiles of a prefix or 1.7 for one, the narrow one's
-// 0.85 for two CTAs; the narrow kernel as a whole is not faster than HBM, 1.25 us per
-// unit and SM; the wide kernel spends 6 us more at its start and end (one B200,
-// D = 128; other head dimensions scale all).
+// then (a little more where it is cut in equal parts). us of an SM per unit of work,
+// side by side on one B200 at D = 128: the wide kernel's 2.5 for two tiles of a prefix
+// or 1.7 for one, the narrow one's 0.85 for two CTAs; the narrow kernel as a whole is
+// not faster than HBM, 1.25 us per unit and SM; the wide kernel spends 6 us more at
+// its start and end. D = 64 goes by the same numbers although they do not scale alike:
+// alone, from D = 128 to 64, the wide kernel's unit goes from 2.15 us to 2.09 (one
+// tile 1.35 to 1.13), the narrow one's from 1.39 to 0.68 from HBM, 0.70 to 0.63 from L2.
 struct WideShare {
   int per, work;
 };

@@ -189,9 +189,13 @@ def attention_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     (`block_table` [batch, columns]), caches [blocks, Hkv, block_rows, D]. The
     prefix is visible to every token; `causal` makes the tokens of a request its
     last cached rows. `max_q_len` is the most tokens a request is expected to
-    have (a hint; by default all of them). Rows of `out` behind q_start[batch]
-    are left as they are; `out` must not overlap an input. `workspace`: a device
-    buffer of attention_paged_workspace_bytes, allocated here if None."""
+    have, a hint that chooses kernels: give 1 for a decode step (by default all the
+    tokens, for which a batch of more than 16 query rows per KV head takes the
+    kernel of prompt chunks). Own rows within a length must be finite where a token
+    may not see them. Rows of `out` outside [q_start[0], q_start[batch]) are left as
+    they are; `out` must not overlap an input. `workspace`: a device buffer of
+    attention_paged_workspace_bytes (44 MB at D = 128, 22 MB at 64, and more with the
+    tokens), allocated here if None."""
     lib = _native.load()
     index, blocks, Hkv, rows, D, stride = _cache(k_cache, v_cache)
     shape, q_stride = query.shape, query.stride()
